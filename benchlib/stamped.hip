@@ -12,6 +12,9 @@
 #include "../tccl_amd/csrc/tree.hip"
 #include "../tccl_amd/csrc/pipeline.hip"
 #include "../tccl_amd/csrc/ipc.hip"
+#include "../tccl_amd/csrc/qk_norm.hip"
+#include "../tccl_amd/csrc/cache.hip"
+#include "../tccl_amd/csrc/attention.hip"
 
 // Device address of the stamp words on the current device, how many 64-bit words a workgroup has
 // and how many workgroups there is room for.

@@ -61,7 +61,8 @@ enum {
 
 typedef enum {
     TCCL_BF16 = 0, /* bf16 in/out, fp32 accumulate, one RNE rounding */
-    TCCL_F32 = 1   /* fp32 in/out, fp32 accumulate */
+    TCCL_F32 = 1,  /* fp32 in/out, fp32 accumulate */
+    TCCL_E4M3 = 2  /* 8-bit storage of a paged cache (OCP e4m3, no infinities); no operand of a collective */
 } tccl_dtype_t;
 
 /* Launch shape override, for tuning and tests.  Any field left 0 is chosen by the
@@ -433,6 +434,83 @@ int tccl_stream_synchronize(void *stream);
 /* Device facts used for reporting: compute units, memory clock (kHz), bus width (bits),
  * L2 bytes.  Any pointer may be NULL. */
 int tccl_device_info(int *compute_units, int *mem_clock_khz, int *mem_bus_bits, size_t *l2_bytes);
+
+/* ------------------------------------------------------------------ attention over ranks
+ * What the ranks of a language model do between their collectives, over the same W source pointers.  head_dim is
+ * 64, 128 or 256 in all of them; pointers to 4- and 8-byte integers, and inv_freq, need their natural alignment
+ * only.  The reference has no counterpart of these.
+ *
+ * tccl_qk_norm_rope: one-shot all-reduce (sum) of `tokens` rows of q_heads + k_heads + v_heads heads whose epilogue
+ * norms each query and key head (x / sqrt(mean x^2 + eps) * weight) and rotates its first rotary_dim elements
+ * (a multiple of 16, at most head_dim) by the angles positions[t] * inv_freq[i], i < rotary_dim / 2.
+ * Pair i is elements (i, i + rotary_dim / 2), or (2i, 2i + 1) if `interleaved`.  The sum, norm and rotation are
+ * fp32 and rounded once.  Outputs are [tokens][heads][head_dim] each; a kind with no heads may have a NULL output. */
+int tccl_qk_norm_rope(const void *const *bufs, int world, void *q_out, void *k_out, void *v_out,
+                      const void *q_weight, const void *k_weight, const int64_t *positions,
+                      const double *inv_freq, size_t tokens, int q_heads, int k_heads, int v_heads,
+                      int head_dim, int rotary_dim, int interleaved, float eps, int dtype, void *stream);
+
+/* Its backward pass: from dq, dk, dv (laid out as the outputs above) and the same sources the gradient dx of
+ * every source (they are equal), [tokens][all heads][head_dim], and of the two weights, in fp32.  The weights'
+ * sums have a fixed order.  `workspace`: tccl_qk_norm_rope_backward_workspace(head_dim) bytes, written before
+ * they are read; not to be shared by calls that may run at the same time. */
+size_t tccl_qk_norm_rope_backward_workspace(int head_dim);
+int tccl_qk_norm_rope_backward(const void *const *bufs, int world, const void *dq, const void *dk,
+                               const void *dv, const void *q_weight, const void *k_weight,
+                               const int64_t *positions, const double *inv_freq, void *dx,
+                               float *dq_weight, float *dk_weight, void *workspace, size_t workspace_bytes,
+                               size_t tokens, int q_heads, int k_heads, int v_heads, int head_dim,
+                               int rotary_dim, int interleaved, float eps, int dtype, void *stream);
+
+/* A paged key/value cache in W buffers of tccl_paged_cache_bytes() each.  Pages are numbered over all ranks:
+ * rank r holds pages [r * pages_per_rank, (r + 1) * pages_per_rank).  A slot is page * page_size + place in the
+ * page.  dtype TCCL_E4M3 keeps every token's head as e4m3 codes times 2^e, e the least exponent >= -110
+ * with 448 * 2^e >= the largest finite magnitude; infinities are kept as NaN.  The layout inside a page is the
+ * library's own. */
+typedef struct {
+    void *bufs[TCCL_MAX_WORLD];
+    int world;
+    int pages_per_rank;
+    int page_size; /* 16, 32, 64, 128 or 256 tokens */
+    int kv_heads;
+    int head_dim;
+    int dtype;     /* TCCL_BF16 or TCCL_E4M3 */
+} tccl_paged_cache;
+
+/* Bytes of one rank's buffer; 0 for a description that is not valid (bufs is not looked at). */
+size_t tccl_paged_cache_bytes(const tccl_paged_cache *cache);
+
+/* Writes k and v [tokens][kv_heads][head_dim] (dtype bf16 or fp32; strides of tokens and heads in elements, whole
+ * 16-byte vectors) at slots[t].  A slot below 0 or outside the pool is not written; slots of one call have to
+ * differ (of two tokens with the same slot either may stay, element by element). */
+int tccl_cache_write(const tccl_paged_cache *cache, const void *k, const void *v, size_t k_token_stride,
+                     size_t k_head_stride, size_t v_token_stride, size_t v_head_stride,
+                     const int64_t *slots, size_t tokens, int dtype, void *stream);
+
+/* Reads slots[t] into k_out and v_out [tokens][kv_heads][head_dim] (dtype bf16 or fp32: both hold the stored
+ * values exactly).  A slot below 0 or outside the pool reads as zeros. */
+int tccl_cache_read(const tccl_paged_cache *cache, const int64_t *slots, size_t tokens, void *k_out,
+                    void *v_out, int dtype, void *stream);
+
+/* Attention of one new token per sequence: q [batch][q_heads][head_dim] bf16 (strides in elements, whole 16-byte
+ * vectors), q_heads a multiple of the cache's kv_heads (query head i reads key head i / (q_heads / kv_heads)).
+ * Token t of sequence b lies on page page_table[b * page_table_stride + t / page_size]; a sequence has
+ * min(lengths[b], max_tokens) tokens, and page_table rows must reach that far.  Tokens on a page
+ * outside the pool are left out.  out [batch][q_heads][head_dim] bf16 and lse [batch][q_heads] (natural log, may
+ * be NULL); without tokens out is 0 and lse -inf.  `workspace`: tccl_decode_attention_workspace() bytes for the same
+ * sizes (may be 0), written before they are read; not to be shared by calls that may run at the same time. */
+size_t tccl_decode_attention_workspace(size_t batch, int q_heads, int kv_heads, int head_dim, int max_tokens);
+int tccl_decode_attention(const tccl_paged_cache *cache, const void *q, size_t q_batch_stride,
+                          size_t q_head_stride, const int32_t *page_table, size_t page_table_stride,
+                          const int32_t *lengths, void *out, float *lse, void *workspace,
+                          size_t workspace_bytes, size_t batch, int q_heads, int max_tokens, float scale,
+                          void *stream);
+
+/* Joins `world` partial attentions over disjoint tokens: out = sum_i w_i outs[i] / sum_i w_i with
+ * w_i = exp(lses[i] - max), lse = max + log sum_i w_i; rows of head_dim elements (dtype bf16 or fp32), lses
+ * fp32.  A source whose lse is -inf is not used; where all are, out is 0 and lse -inf. */
+int tccl_attention_all_reduce(const void *const *outs, const void *const *lses, int world, void *out,
+                              float *lse, size_t rows, int head_dim, int dtype, void *stream);
 
 #ifdef __cplusplus
 }

@@ -7,6 +7,8 @@ from .collectives import (DoubleTreePlan, all_gather, all_reduce, double_tree_al
                           one_shot_all_reduce, one_shot_reduce_scatter, reduce_scatter, signal_pad_timeouts, two_shot_all_reduce,
                           two_shot_all_reduce_world)
 from .symm import SymmGroup, SymmHandle, empty_world, register, rendezvous, unregister
+from .attention import (PagedCache, attention_all_reduce, cache_read, cache_write, decode_attention, qk_norm_rope,
+                        qk_norm_rope_backward)
 from . import ipc, spmd, tree
 from .tree import build_double_tree, build_tree, get_parents_and_children
 
@@ -14,6 +16,7 @@ __all__ = [
     "LaunchCfg", "TcclError", "load_library",
     "one_shot_all_reduce", "one_shot_reduce_scatter", "one_shot_all_gather", "double_tree_all_reduce",
     "double_tree_all_reduce_world", "signal_pad_timeouts", "two_shot_all_reduce_world", "DoubleTreePlan", "reduce_scatter", "all_gather", "two_shot_all_reduce", "all_reduce",
+    "qk_norm_rope", "qk_norm_rope_backward", "PagedCache", "cache_write", "cache_read", "decode_attention", "attention_all_reduce",
     "SymmGroup", "SymmHandle", "empty_world", "register", "rendezvous", "unregister",
     "ipc", "spmd", "tree", "build_tree", "build_double_tree", "get_parents_and_children",
 ]

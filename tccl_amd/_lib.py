@@ -20,6 +20,7 @@ IPC_HANDLE_BYTES = 64
 
 TCCL_BF16 = 0
 TCCL_F32 = 1
+TCCL_E4M3 = 2
 
 CFG_NONTEMPORAL_LOAD = 1
 CFG_NONTEMPORAL_STORE = 2
@@ -59,11 +60,20 @@ class NodeJob(ctypes.Structure):
                 ("is_copy", ctypes.c_int), ("pad_", ctypes.c_int)]
 
 
+class PagedCacheDesc(ctypes.Structure):
+    """Mirror of ``tccl_paged_cache``."""
+    _fields_ = [("bufs", ctypes.c_void_p * MAX_WORLD), ("world", ctypes.c_int), ("pages_per_rank", ctypes.c_int),
+                ("page_size", ctypes.c_int), ("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int),
+                ("dtype", ctypes.c_int)]
+
+
 _P = ctypes.c_void_p
 _PP = ctypes.POINTER(ctypes.c_void_p)
 _SZ = ctypes.c_size_t
 _I = ctypes.c_int
 _CFG = ctypes.POINTER(LaunchCfg)
+_CACHE = ctypes.POINTER(PagedCacheDesc)
+_F = ctypes.c_float
 
 # name -> (restype, argtypes); exactly the symbols include/tccl_amd.h declares.
 SIGNATURES = {
@@ -106,6 +116,16 @@ SIGNATURES = {
     "tccl_double_tree_plan_create": (_I, [_PP, _PP, _I, _SZ, _I, _SZ, _PP]),
     "tccl_plan_launch": (_I, [_P, _P]),
     "tccl_plan_destroy": (_I, [_P]),
+    "tccl_qk_norm_rope": (_I, [_PP, _I, _P, _P, _P, _P, _P, _P, _P, _SZ, _I, _I, _I, _I, _I, _I, _F, _I, _P]),
+    "tccl_qk_norm_rope_backward_workspace": (_SZ, [_I]),
+    "tccl_qk_norm_rope_backward": (_I, [_PP, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _SZ, _I, _I, _I, _I,
+                                        _I, _I, _F, _I, _P]),
+    "tccl_paged_cache_bytes": (_SZ, [_CACHE]),
+    "tccl_cache_write": (_I, [_CACHE, _P, _P, _SZ, _SZ, _SZ, _SZ, _P, _SZ, _I, _P]),
+    "tccl_cache_read": (_I, [_CACHE, _P, _SZ, _P, _P, _I, _P]),
+    "tccl_decode_attention_workspace": (_SZ, [_SZ, _I, _I, _I, _I]),
+    "tccl_decode_attention": (_I, [_CACHE, _P, _SZ, _SZ, _P, _SZ, _P, _P, _P, _P, _SZ, _SZ, _I, _I, _F, _P]),
+    "tccl_attention_all_reduce": (_I, [_PP, _PP, _I, _P, _P, _SZ, _I, _I, _P]),
     "tccl_event_create": (_I, [_PP]),
     "tccl_event_destroy": (_I, [_P]),
     "tccl_event_record": (_I, [_P, _P]),

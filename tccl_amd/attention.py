@@ -1,0 +1,344 @@
+"""What the ranks of a language model do between their collectives, over the same W symmetric buffers:
+
+* ``qk_norm_rope`` / ``qk_norm_rope_backward`` -- one-shot all-reduce of the ranks' partial query/key/value
+  projections with the per-head norms and the position rotation in the same pass, and its gradients;
+* ``PagedCache``, ``cache_write``, ``cache_read`` -- a paged key/value cache that spans the ranks, in bf16 or 8 bits;
+* ``decode_attention`` -- one new token per sequence attends to pages on all ranks;
+* ``attention_all_reduce`` -- where each rank attends to its own part of the tokens, the join of the W partial
+  attentions: an all-reduce whose weights are a softmax over the ranks.
+
+As in ``collectives``: arguments are checked on the host before anything is launched, outputs are allocated with
+torch unless the caller passes them, kernels run on torch's current stream of the tensors' device, nothing
+synchronises, and every call can be captured into a HIP graph.  Inside ``spmd.run`` every rank makes the call,
+except ``cache_write``, which a rank may make alone.  None of these functions records anything for autograd.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+import math
+from typing import Optional, Tuple, Union
+
+import torch
+
+from . import _lib, spmd
+from .collectives import _check_out, _refuse_remote, _stream, _sum_dtype
+from .symm import rendezvous, SymmGroup
+
+HEAD_DIMS = (64, 128, 256)
+PAGE_SIZES = (16, 32, 64, 128, 256)
+_STORES = {torch.bfloat16: _lib.TCCL_BF16, torch.float8_e4m3fn: _lib.TCCL_E4M3}
+
+
+def _on(device: torch.device):
+    """Launches go to the device of the tensors, whichever is current."""
+    if device.type != "cuda":
+        raise ValueError(f"the kernels take tensors on a GPU, not on {device}")
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _need(condition: bool, text: str) -> None:
+    if not condition:
+        raise ValueError(text)
+
+
+def _integers(t: torch.Tensor, dtype: torch.dtype, shape, device: torch.device, name: str) -> None:
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {device}")
+
+
+def _aligned(t: torch.Tensor, name: str) -> None:
+    if t.data_ptr() % 16:
+        raise ValueError(f"{name} must start at a multiple of 16 bytes")
+
+
+def _heads_first(t: torch.Tensor, name: str) -> Tuple[int, int]:
+    """Strides (in elements) of a ``[tokens, heads, head_dim]`` tensor whose rows are whole and 16-byte aligned."""
+    vec = 16 // t.element_size()
+    token, head = t.stride(0), t.stride(1)
+    if t.numel() and (t.stride(2) != 1 or token < 0 or head < 0 or token % vec or head % vec or t.data_ptr() % 16):
+        raise ValueError(f"{name}: rows of head_dim elements must be contiguous and start at multiples of 16 bytes")
+    return (token, head) if t.numel() else (0, 0)
+
+
+# ---------------------------------------------------------------- sum, per-head norm and rotation
+
+def _norm_arguments(tensor, q_weight, k_weight, positions, inv_freq, heads, what):
+    dtype = _sum_dtype(tensor)
+    dim = q_weight.numel()
+    _need(dim in HEAD_DIMS, f"{what}: head_dim (the weights' length) must be one of {HEAD_DIMS}")
+    _need(tensor.dim() == 2, f"{what}: the projection must be [tokens, columns]")
+    device = tensor.device
+    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        if w.dtype != tensor.dtype or w.shape != (dim,) or w.device != device or not w.is_contiguous():
+            raise ValueError(f"{what}: {name} must be a contiguous {tensor.dtype} tensor of shape ({dim},) on {device}")
+        _aligned(w, name)
+    tokens, columns = tensor.shape
+    _need(all(n >= 0 for n in heads) and sum(heads) >= 1 and sum(heads) * dim == columns,
+          f"{what}: {columns} columns are not {heads[0]} + {heads[1]} + {heads[2]} heads of {dim}")
+    _integers(positions, torch.int64, (tokens,), device, "positions")
+    if inv_freq.dim() != 1 or inv_freq.dtype != torch.float64 or inv_freq.device != device or not inv_freq.is_contiguous():
+        raise ValueError(f"{what}: inv_freq must be a contiguous float64 vector on {device}")
+    rotary = 2 * inv_freq.numel()
+    _need(rotary % 16 == 0 and rotary <= dim, f"{what}: 2 * len(inv_freq) must be a multiple of 16 and at most head_dim")
+    return dtype, dim, rotary
+
+
+def qk_norm_rope(tensor: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, positions: torch.Tensor,
+                 inv_freq: torch.Tensor, q_heads: int, k_heads: int, *, eps: float = 1e-6,
+                 interleaved: bool = False) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """All-reduce (sum) of the ranks' partial projections, then each query and key head normed and rotated.
+
+    ``tensor`` is this rank's ``[tokens, columns]`` buffer (bfloat16 or float32) of a symmetric group, columns holding
+    ``q_heads`` query heads, ``k_heads`` key heads and, in what is left, value heads, of ``len(q_weight)`` elements
+    each (64, 128 or 256).  A query or key head becomes ``R(position) (x / sqrt(mean(x^2) + eps) * weight)``, where R
+    turns the first ``2 * len(inv_freq)`` elements (a multiple of 16) in pairs (i, i + half), or (2i, 2i + 1) if
+    ``interleaved``, by ``positions[t] * inv_freq[i]``: positions are int64, inv_freq float64, and the angle is reduced
+    in fp64, so that far positions keep their precision.  Value heads are only summed.  Everything is fp32 and rounded
+    once.  Returns q, k, v as ``[tokens, heads, head_dim]``.
+
+    With a group of one rank it is the plain norm and rotation."""
+    dim = q_weight.numel()
+    v_heads = tensor.shape[-1] // max(dim, 1) - q_heads - k_heads
+    heads = (q_heads, k_heads, v_heads)
+    dtype, dim, rotary = _norm_arguments(tensor, q_weight, k_weight, positions, inv_freq, heads, "qk_norm_rope")
+    lib = _lib.load()
+    with spmd.collective():
+        tokens = tensor.shape[0]
+        outs = [torch.empty((tokens, n, dim), dtype=tensor.dtype, device=tensor.device) for n in heads]
+        if tokens == 0:                # (an empty view has no address to find a group by)
+            return outs[0], outs[1], outs[2]
+        symm = rendezvous(tensor)
+        _refuse_remote(symm.group, "qk_norm_rope")
+        symm.group.check_signals()
+        with _on(tensor.device):
+            rc = lib.tccl_qk_norm_rope(symm.buffer_ptrs_host, symm.world_size, *(o.data_ptr() or None for o in outs),
+                                       q_weight.data_ptr(), k_weight.data_ptr(), positions.data_ptr(),
+                                       inv_freq.data_ptr() or None, tokens, *heads, dim, rotary, int(interleaved), eps,
+                                       dtype, _stream(tensor.device))
+        _lib.check("tccl_qk_norm_rope", rc)
+    return outs[0], outs[1], outs[2]
+
+
+def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor, dv: torch.Tensor, tensor: torch.Tensor,
+                          q_weight: torch.Tensor, k_weight: torch.Tensor, positions: torch.Tensor,
+                          inv_freq: torch.Tensor, *, eps: float = 1e-6, interleaved: bool = False
+                          ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Gradients of ``qk_norm_rope`` from the gradients of its three outputs (contiguous ``[tokens, heads, head_dim]``
+    in ``tensor``'s dtype) and its inputs, whose buffers must still hold the partial projections (the sum, norm and
+    rotation angles are formed again; nothing is kept from the forward pass).
+
+    Returns ``(dx, dq_weight, dk_weight)``: dx ``[tokens, columns]`` in ``tensor``'s dtype is the gradient of every
+    rank's buffer alike; the weights' gradients are float32, summed in a fixed order."""
+    heads = tuple(g.shape[1] if g.dim() == 3 else -1 for g in (dq, dk, dv))
+    dtype, dim, rotary = _norm_arguments(tensor, q_weight, k_weight, positions, inv_freq, heads, "qk_norm_rope_backward")
+    tokens = tensor.shape[0]
+    for g, n, name in zip((dq, dk, dv), heads, ("dq", "dk", "dv")):
+        if g.shape != (tokens, n, dim) or g.dtype != tensor.dtype or g.device != tensor.device or not g.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous {tensor.dtype} tensor of shape {(tokens, n, dim)} on {tensor.device}")
+        if g.numel():
+            _aligned(g, name)
+    lib = _lib.load()
+    with spmd.collective():
+        device = tensor.device
+        dx = torch.empty_like(tensor)
+        if tokens == 0:
+            return dx, torch.zeros(dim, device=device), torch.zeros(dim, device=device)
+        symm = rendezvous(tensor)
+        _refuse_remote(symm.group, "qk_norm_rope_backward")
+        symm.group.check_signals()
+        dweights = torch.empty((2, dim), dtype=torch.float32, device=device)
+        with _on(device):
+            nbytes = lib.tccl_qk_norm_rope_backward_workspace(dim)
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            first = dweights.data_ptr()
+            rc = lib.tccl_qk_norm_rope_backward(
+                symm.buffer_ptrs_host, symm.world_size, *(g.data_ptr() or None for g in (dq, dk, dv)), q_weight.data_ptr(),
+                k_weight.data_ptr(), positions.data_ptr(), inv_freq.data_ptr() or None, dx.data_ptr(), first, first + 4 * dim,
+                workspace.data_ptr(), nbytes, tokens, *heads, dim, rotary, int(interleaved), eps, dtype, _stream(device))
+        _lib.check("tccl_qk_norm_rope_backward", rc)
+    return dx, dweights[0], dweights[1]
+
+
+# ---------------------------------------------------------------- the paged cache
+
+class PagedCache:
+    """A paged key/value cache that spans the ranks: W symmetric buffers (``group``) of ``pages_per_rank`` pages of
+    ``page_size`` tokens (16, 32, 64, 128 or 256).  Pages are numbered over all ranks, rank r holding pages
+    ``[r * pages_per_rank, (r + 1) * pages_per_rank)``; a *slot* is ``page * page_size + place in the page``.  Which
+    sequence has which pages, on which ranks, is the caller's table.
+
+    ``dtype``: ``torch.bfloat16``, or ``torch.float8_e4m3fn`` with one power-of-two scale per token and head, formed as
+    the token is written; stored values are bfloat16 numbers either way.  The layout inside a page is the library's own.
+    A new cache holds zeros."""
+
+    def __init__(self, world_size: int, pages_per_rank: int, page_size: int, kv_heads: int, head_dim: int, *,
+                 dtype: torch.dtype = torch.bfloat16, device="cuda"):
+        _need(1 <= world_size <= _lib.MAX_WORLD, f"world_size must be 1 to {_lib.MAX_WORLD}")
+        _need(dtype in _STORES, "a paged cache holds torch.bfloat16 or torch.float8_e4m3fn")
+        _need(head_dim in HEAD_DIMS, f"head_dim must be one of {HEAD_DIMS}")
+        _need(page_size in PAGE_SIZES, f"page_size must be one of {PAGE_SIZES}")
+        _need(1 <= kv_heads <= 65535, "kv_heads must be 1 to 65535")
+        _need(pages_per_rank >= 1 and pages_per_rank * world_size < 1 << 31, "page numbers must fit 31 bits")
+        self.world_size, self.pages_per_rank, self.page_size = world_size, pages_per_rank, page_size
+        self.kv_heads, self.head_dim, self.dtype = kv_heads, head_dim, dtype
+        self.pages = world_size * pages_per_rank
+        self.slots = self.pages * page_size
+        desc = _lib.PagedCacheDesc()
+        desc.world, desc.pages_per_rank, desc.page_size = world_size, pages_per_rank, page_size
+        desc.kv_heads, desc.head_dim, desc.dtype = kv_heads, head_dim, _STORES[dtype]
+        nbytes = _lib.load().tccl_paged_cache_bytes(ctypes.byref(desc))
+        # a group of its own, but not one that rendezvous finds: its buffers are no operand of a collective
+        self.group = SymmGroup([torch.zeros(nbytes, dtype=torch.uint8, device=device) for _ in range(world_size)])
+        self.device = self.group.tensors[0].device
+        for r, p in enumerate(self.group.buffer_ptrs):
+            desc.bufs[r] = p
+        self._desc = desc
+        self._ref = ctypes.byref(desc)
+
+    def _rows(self, tokens: int) -> Tuple[int, int, int]:
+        return tokens, self.kv_heads, self.head_dim
+
+
+def cache_write(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+    """Write keys and values ``[tokens, kv_heads, head_dim]`` (bfloat16 or float32; any token and head strides of whole
+    16-byte vectors) into the cache at ``slots`` (int64).  A negative slot, or one outside the cache, is not written
+    (padding); the slots of one call must differ from each other."""
+    dtype = _sum_dtype(k)
+    tokens = slots.numel()
+    for t, name in ((k, "k"), (v, "v")):
+        if t.shape != cache._rows(tokens) or t.dtype != k.dtype or t.device != cache.device:
+            raise ValueError(f"{name} must be a {k.dtype} tensor of shape {cache._rows(tokens)} on {cache.device}")
+    strides = _heads_first(k, "k") + _heads_first(v, "v")
+    _integers(slots, torch.int64, (tokens,), cache.device, "slots")
+    if tokens == 0:
+        return
+    with _on(cache.device):
+        rc = _lib.load().tccl_cache_write(cache._ref, k.data_ptr(), v.data_ptr(), *strides, slots.data_ptr(), tokens,
+                                          dtype, _stream(cache.device))
+    _lib.check("tccl_cache_write", rc)
+
+
+def cache_read(cache: PagedCache, slots: torch.Tensor, *, dtype: torch.dtype = torch.bfloat16,
+               out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Keys and values at ``slots`` (int64, any order, repeats allowed) as two ``[tokens, kv_heads, head_dim]`` tensors of
+    ``dtype`` (bfloat16 or float32; both hold the stored values exactly): a gather over the ranks.  A negative slot, or
+    one outside the cache, reads as zeros."""
+    tokens = slots.numel()
+    _integers(slots, torch.int64, (tokens,), cache.device, "slots")
+    _need(dtype in (torch.bfloat16, torch.float32), "cache_read returns bfloat16 or float32")
+    if out is None:
+        k, v = (torch.empty(cache._rows(tokens), dtype=dtype, device=cache.device) for _ in range(2))
+    else:
+        k, v = out
+        for t, name in ((k, "out[0]"), (v, "out[1]")):
+            if t.shape != cache._rows(tokens) or t.dtype != dtype or t.device != cache.device or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {cache._rows(tokens)} on {cache.device}")
+    code = _sum_dtype(k)
+    with spmd.collective():
+        if tokens:
+            _aligned(k, "out[0]")
+            _aligned(v, "out[1]")
+            with _on(cache.device):
+                rc = _lib.load().tccl_cache_read(cache._ref, slots.data_ptr(), tokens, k.data_ptr(), v.data_ptr(), code,
+                                                 _stream(cache.device))
+            _lib.check("tccl_cache_read", rc)
+    return k, v
+
+
+# ---------------------------------------------------------------- attention
+
+def decode_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor, lengths: torch.Tensor, *,
+                     scale: Optional[float] = None, max_length: Optional[int] = None, return_lse: bool = False,
+                     out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None
+                     ) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """Attention of one new token per sequence over the cached tokens of all ranks.
+
+    ``q``: ``[batch, q_heads, head_dim]`` bfloat16 (any strides of whole 16-byte vectors), q_heads a multiple of the
+    cache's kv_heads; query head i reads key head ``i // (q_heads // kv_heads)``.  ``page_table``: int32 ``[batch, pages]``
+    (rows may be strided), page numbers of each sequence in order; ``lengths``: int32 ``[batch]``, how many tokens each
+    has.  Entries behind a sequence's last page are not looked at, and tokens on a page number outside the cache are
+    left out.  ``max_length``: an upper bound of the lengths that the host knows (default: what the table has room for);
+    the launch is shaped for it, and tokens beyond it are left out.
+
+    Returns ``[batch, q_heads, head_dim]`` bfloat16 and, with ``return_lse`` or ``lse``, the logarithm of the softmax's
+    sum, float32 ``[batch, q_heads]``: what ``attention_all_reduce`` joins parts with.  A sequence without tokens gives
+    0 and -inf.  Scores, softmax and sums are fp32; an infinite cached value gives NaN."""
+    batch = lengths.numel()
+    dim = cache.head_dim
+    _need(q.dtype == torch.bfloat16, "decode_attention takes bfloat16 queries")
+    if q.dim() != 3 or q.shape[0] != batch or q.shape[2] != dim or q.device != cache.device:
+        raise ValueError(f"q must be [{batch}, q_heads, {dim}] on {cache.device}")
+    q_heads = q.shape[1]
+    _need(q_heads >= 1 and q_heads % cache.kv_heads == 0, "q_heads must be a multiple of the cache's kv_heads")
+    q_strides = _heads_first(q, "q")
+    _integers(lengths, torch.int32, (batch,), cache.device, "lengths")
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != batch \
+            or page_table.device != cache.device:
+        raise ValueError(f"page_table must be an int32 tensor of shape [{batch}, pages] on {cache.device}")
+    width = page_table.shape[1]
+    _need(width <= 1 or page_table.stride(1) == 1, "page_table: a row must be contiguous")
+    _need(page_table.stride(0) >= 0, "page_table: rows must be in ascending order")
+    most = width * cache.page_size
+    if max_length is not None:
+        _need(max_length >= 0, "max_length must not be negative")
+        most = min(most, max_length)
+    _need(most < 1 << 31, "page_table has room for more than 2^31 tokens")
+    device = cache.device
+    shape = (batch, q_heads, dim)
+    out = torch.empty(shape, dtype=torch.bfloat16, device=device) if out is None else _check_out(out, shape, q)
+    if lse is not None:
+        _integers(lse, torch.float32, (batch, q_heads), device, "lse")
+    elif return_lse:
+        lse = torch.empty((batch, q_heads), dtype=torch.float32, device=device)
+    lib = _lib.load()
+    if scale is None:
+        scale = 1.0 / math.sqrt(dim)
+    with spmd.collective():
+        if batch:
+            _aligned(out, "out")
+            with _on(device):
+                nbytes = lib.tccl_decode_attention_workspace(batch, q_heads, cache.kv_heads, dim, most)
+                workspace = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+                rc = lib.tccl_decode_attention(
+                    cache._ref, q.data_ptr(), *q_strides, page_table.data_ptr() or None, page_table.stride(0),
+                    lengths.data_ptr(), out.data_ptr(), lse.data_ptr() if lse is not None else None,
+                    workspace.data_ptr() if nbytes else None, nbytes, batch, q_heads, most, scale, _stream(device))
+            _lib.check("tccl_decode_attention", rc)
+    return (out, lse) if lse is not None else out
+
+
+def attention_all_reduce(tensor: torch.Tensor, lse: torch.Tensor, *, out: Optional[torch.Tensor] = None
+                         ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Join of the ranks' partial attentions over disjoint parts of the tokens: an all-reduce
+    ``sum_i w_i tensor_i / sum_i w_i`` with ``w_i = exp(lse_i - max)``, beside ``one_shot_all_reduce``.
+
+    ``tensor``: this rank's ``[..., head_dim]`` buffer (bfloat16 or float32, head_dim 64, 128 or 256) of one symmetric
+    group, ``lse``: its float32 ``[...]`` buffer of another, both as ``decode_attention(out=, lse=)`` fills them.  Returns
+    the joined output and its lse, the same on every rank.  A rank whose lse is -inf is left out, whatever its buffer
+    holds; where all are, the output is 0 and lse -inf."""
+    dtype = _sum_dtype(tensor)
+    _need(tensor.dim() >= 1 and tensor.shape[-1] in HEAD_DIMS, f"attention_all_reduce: head_dim must be one of {HEAD_DIMS}")
+    if lse.dtype != torch.float32 or lse.shape != tensor.shape[:-1] or lse.device != tensor.device:
+        raise ValueError(f"lse must be a float32 tensor of shape {tuple(tensor.shape[:-1])} on {tensor.device}")
+    lib = _lib.load()
+    with spmd.collective():
+        if lse.numel() == 0:           # (an empty view has no address to find a group by)
+            return torch.empty_like(tensor) if out is None else _check_out(out, tensor.shape, tensor), torch.empty_like(lse)
+        symm, symm_lse = rendezvous(tensor), rendezvous(lse)
+        _refuse_remote(symm.group, "attention_all_reduce")
+        _refuse_remote(symm_lse.group, "attention_all_reduce")
+        _need(symm.world_size == symm_lse.world_size and symm.rank == symm_lse.rank,
+              "attention_all_reduce: tensor and lse must be the same rank's buffers of two groups of one world")
+        symm.group.check_signals()
+        output = torch.empty_like(tensor) if out is None else _check_out(out, tensor.shape, tensor)
+        output_lse = torch.empty_like(lse)
+        _aligned(output, "out")
+        with _on(tensor.device):
+            rc = lib.tccl_attention_all_reduce(symm.buffer_ptrs_host, symm_lse.buffer_ptrs_host, symm.world_size,
+                                               output.data_ptr(), output_lse.data_ptr(), lse.numel(),
+                                               tensor.shape[-1], dtype, _stream(tensor.device))
+        _lib.check("tccl_attention_all_reduce", rc)
+    return output, output_lse

@@ -1,0 +1,461 @@
+// qk_norm.hip -- a one-shot all-reduce of the ranks' partial query/key/value projections whose epilogue
+// norms every query and key head and rotates it by its token's position, and its backward pass.
+//
+//   x = sum_i buf_i            fp32, rank order; a head is head_dim consecutive elements
+//   r = 1 / sqrt(mean x^2 + eps),  n = x r,  h = n w          (q_weight for query heads, k_weight for key heads)
+//   y = R(position) h          pairs (a, b) -> (a cos - b sin, b cos + a sin), angle position * inv_freq[i]
+// value heads behind the keys are only summed.  Backward, with g = R^T dy, u = g w:
+//   dx = r (u - n mean(u n)),  dw = sum over tokens and heads of g n
+//
+// Memory-bound: W reads and one write per element, a few dozen operations each.  A lane holds eight
+// elements, so a wave works on 512 consecutive elements (four heads of 128) with one 16-byte load per
+// source; the mean is a reduction over head_dim / 8 lanes in registers.  Angles are formed in fp64 turns
+// (fp32 would lose the fraction of a far position's angle) once per token by the workgroup, into LDS.
+#include "host.h"
+#include "rows.h"
+
+namespace tccl {
+
+constexpr int kNormBlock = 256;
+constexpr int kNormWaves = kNormBlock / 64;
+constexpr int kNormTokens = 4; // most tokens a workgroup works on at once
+constexpr int kMaxRotary = 256;
+
+template <int NSRC>
+struct NormArgs {
+    const char *src[NSRC];
+    char *out[3];        // forward: q, k, v;  backward: dx, unused, unused
+    const char *grad[3]; // backward: dq, dk, dv
+    const char *weight[2];
+    const int64_t *positions;
+    const double *inv_freq;
+    float *partial; // backward: [workgroups][2][head_dim] sums of g n
+    size_t tokens;
+    int heads[3];
+    int rotary, interleaved;
+    int tokens_per_wg; // 1, 2 or 4
+    float eps;
+};
+
+// cos and sin of position * inv_freq[i].  The angle is reduced to (-1/2, 1/2] turns in fp64.
+__device__ __forceinline__ f32x2 rotation(int64_t position, double inv_freq)
+{
+    double turns = static_cast<double>(position) * inv_freq * 0.15915494309189533577;
+    turns = turns - __builtin_rint(turns);
+    const float half_turns = static_cast<float>(turns + turns);
+    return f32x2{cospif(half_turns), sinpif(half_turns)};
+}
+
+// A lane's eight elements, rotated (SIGN = 1) or rotated back (-1); `place` is the lane's place in its row.
+template <int LANES, int SIGN>
+__device__ __forceinline__ void rotate(float *x, const f32x2 *turn, int place, int rotary, bool interleaved)
+{
+    const int lanes = rotary >> 3;
+    if (interleaved) {
+        if (place < lanes) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const f32x2 cs = turn[4 * place + k];
+                const float s = SIGN * cs.y, a = x[2 * k], b = x[2 * k + 1];
+                x[2 * k] = __builtin_fmaf(a, cs.x, -(b * s));
+                x[2 * k + 1] = __builtin_fmaf(b, cs.x, a * s);
+            }
+        }
+    } else {
+        const int half = lanes >> 1;
+        const bool low = place < half;
+        const int other = place >= lanes ? place : (low ? place + half : place - half);
+        const int lane = threadIdx.x & 63;
+        const int from = (lane & ~(LANES - 1)) + other;
+        float y[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) y[k] = __shfl(x[k], from);
+        if (place < lanes) {
+            const f32x2 *t = turn + 8 * (low ? place : place - half);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const f32x2 cs = t[k];
+                const float s = SIGN * (low ? -cs.y : cs.y);
+                x[k] = __builtin_fmaf(x[k], cs.x, y[k] * s);
+            }
+        }
+    }
+}
+
+template <class Row, int NSRC>
+__device__ __forceinline__ void sum_sources(const Row *in, float *x)
+{
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        float a = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NSRC; ++i) a = a + in[i].at(k);
+        x[k] = a;
+    }
+}
+
+template <int LANES>
+__device__ __forceinline__ float inverse_rms(const float *x, float eps)
+{
+    float s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s = __builtin_fmaf(x[k], x[k], s);
+    return rsqrtf(__builtin_fmaf(reduce_row<AddOp, LANES>(s), 1.0f / (8 * LANES), eps));
+}
+
+// The angles of the workgroup's tokens, [token][rotary / 2].
+template <int NSRC>
+__device__ __forceinline__ void fill_angles(const NormArgs<NSRC> &a, f32x2 *turn, size_t first)
+{
+    const int half = a.rotary >> 1;
+    for (int i = threadIdx.x; i < half * a.tokens_per_wg; i += kNormBlock) {
+        const size_t t = first + i / half;
+        if (t < a.tokens) turn[i] = rotation(a.positions[t], a.inv_freq[i % half]);
+    }
+}
+
+template <class Row, int LANES, int NSRC>
+__global__ void __launch_bounds__(kNormBlock)
+qk_norm_rope_kernel(NormArgs<NSRC> a)
+{
+    constexpr int D = 8 * LANES, HEADS = 64 / LANES; // heads a wave holds
+    __shared__ f32x2 turn[kNormTokens * kMaxRotary / 2];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, place = lane & (LANES - 1);
+    const int all = a.heads[0] + a.heads[1] + a.heads[2];
+    const int groups = (all + HEADS - 1) / HEADS;
+    const size_t first = static_cast<size_t>(blockIdx.x) * a.tokens_per_wg;
+    float wq[8], wk[8];
+    load_row<Row>(a.weight[0] + place * 8 * Row::kElemBytes, wq);
+    load_row<Row>(a.weight[1] + place * 8 * Row::kElemBytes, wk);
+    fill_angles(a, turn, first);
+    __syncthreads();
+    for (int item = wave; item < groups * a.tokens_per_wg; item += kNormWaves) {
+        const int local = item / groups;
+        const size_t token = first + local;
+        const int head = (item - local * groups) * HEADS + lane / LANES;
+        const bool live = token < a.tokens && head < all;
+        const size_t at = ((token * all + head) * D + place * 8) * Row::kElemBytes;
+        Row in[NSRC];
+#pragma unroll
+        for (int i = 0; i < NSRC; ++i) {
+            if (live)
+                in[i].load(a.src[i] + at);
+            else
+                in[i].zero();
+        }
+        float x[8];
+        sum_sources<Row, NSRC>(in, x);
+        const float r = inverse_rms<LANES>(x, a.eps);
+        const bool is_q = head < a.heads[0], is_v = head >= a.heads[0] + a.heads[1];
+        float y[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) y[k] = x[k] * r * (is_q ? wq[k] : wk[k]);
+        rotate<LANES, 1>(y, turn + local * (a.rotary >> 1), place, a.rotary, a.interleaved != 0);
+        if (is_v) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) y[k] = x[k];
+        }
+        if (live) {
+            const int kind = is_q ? 0 : (is_v ? 2 : 1);
+            const int before = is_q ? 0 : (is_v ? a.heads[0] + a.heads[1] : a.heads[0]);
+            char *out = is_q ? a.out[0] : (is_v ? a.out[2] : a.out[1]);
+            const int mine = is_q ? a.heads[0] : (kind == 2 ? a.heads[2] : a.heads[1]);
+            Row::store(out + ((token * mine + (head - before)) * D + place * 8) * Row::kElemBytes, y);
+        }
+    }
+}
+
+// Workgroups walk the tokens with the grid's stride; each lane keeps the weight gradients of its eight dims
+// in registers until the end, so that a workgroup leaves one partial row and the result does not depend on
+// the order in which workgroups finish.
+template <class Row, int LANES, int NSRC>
+__global__ void __launch_bounds__(kNormBlock)
+qk_norm_rope_backward_kernel(NormArgs<NSRC> a)
+{
+    constexpr int D = 8 * LANES, HEADS = 64 / LANES;
+    __shared__ f32x2 turn[kNormTokens * kMaxRotary / 2];
+    __shared__ float sums[kNormWaves][2][D];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, place = lane & (LANES - 1);
+    const int all = a.heads[0] + a.heads[1] + a.heads[2];
+    const int groups = (all + HEADS - 1) / HEADS;
+    float wq[8], wk[8];
+    load_row<Row>(a.weight[0] + place * 8 * Row::kElemBytes, wq);
+    load_row<Row>(a.weight[1] + place * 8 * Row::kElemBytes, wk);
+    float dw[2][8] = {};
+    for (size_t first = static_cast<size_t>(blockIdx.x) * a.tokens_per_wg; first < a.tokens;
+         first += static_cast<size_t>(gridDim.x) * a.tokens_per_wg) {
+        fill_angles(a, turn, first);
+        __syncthreads();
+        for (int item = wave; item < groups * a.tokens_per_wg; item += kNormWaves) {
+            const int local = item / groups;
+            const size_t token = first + local;
+            const int head = (item - local * groups) * HEADS + lane / LANES;
+            const bool live = token < a.tokens && head < all;
+            const bool is_q = head < a.heads[0], is_v = head >= a.heads[0] + a.heads[1];
+            const int before = is_q ? 0 : (is_v ? a.heads[0] + a.heads[1] : a.heads[0]);
+            const int mine = is_q ? a.heads[0] : (is_v ? a.heads[2] : a.heads[1]);
+            const char *dy = is_q ? a.grad[0] : (is_v ? a.grad[2] : a.grad[1]);
+            const size_t at = ((token * all + head) * D + place * 8) * Row::kElemBytes;
+            Row in[NSRC], dg;
+#pragma unroll
+            for (int i = 0; i < NSRC; ++i) {
+                if (live && !is_v)
+                    in[i].load(a.src[i] + at);
+                else
+                    in[i].zero();
+            }
+            if (live)
+                dg.load(dy + ((token * mine + (head - before)) * D + place * 8) * Row::kElemBytes);
+            else
+                dg.zero();
+            float x[8], g[8];
+            sum_sources<Row, NSRC>(in, x);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) g[k] = dg.at(k);
+            const float r = inverse_rms<LANES>(x, a.eps);
+            rotate<LANES, -1>(g, turn + local * (a.rotary >> 1), place, a.rotary, a.interleaved != 0);
+            float dot = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float n = x[k] * r, gn = g[k] * n;
+                dot = __builtin_fmaf(gn, is_q ? wq[k] : wk[k], dot);
+                // a value head's (and a missing head's) x is zero here, and so is its gn
+                dw[0][k] = dw[0][k] + (is_q ? gn : 0.0f);
+                dw[1][k] = dw[1][k] + (is_q || is_v ? 0.0f : gn);
+            }
+            dot = reduce_row<AddOp, LANES>(dot) * (1.0f / D);
+            float d[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float n = x[k] * r, u = g[k] * (is_q ? wq[k] : wk[k]);
+                d[k] = is_v ? dg.at(k) : r * __builtin_fmaf(-n, dot, u);
+            }
+            if (live) Row::store(a.out[0] + at, d);
+        }
+        __syncthreads();
+    }
+    // over the wave's heads (lanes LANES apart), then over the waves
+#pragma unroll
+    for (int kind = 0; kind < 2; ++kind) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            float s = dw[kind][k];
+#pragma unroll
+            for (int step = LANES; step < 64; step *= 2) s = s + __shfl_xor(s, step);
+            if (lane < LANES) sums[wave][kind][place * 8 + k] = s;
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * D; i += kNormBlock) {
+        float s = 0.0f;
+#pragma unroll
+        for (int v = 0; v < kNormWaves; ++v) s = s + (&sums[v][0][0])[i];
+        a.partial[static_cast<size_t>(blockIdx.x) * 2 * D + i] = s;
+    }
+}
+
+// The partial rows in order: 16 columns per workgroup, 16 row lanes each, joined through LDS.
+__global__ void __launch_bounds__(256)
+weight_grad_kernel(const float *partial, int rows, int dim, float *dq_weight, float *dk_weight)
+{
+    __shared__ float part[16][17];
+    const int column = blockIdx.x * 16 + (threadIdx.x & 15), lane = threadIdx.x >> 4;
+    float s = 0.0f;
+    for (int r = lane; r < rows; r += 16) s = s + partial[static_cast<size_t>(r) * 2 * dim + column];
+    part[lane][threadIdx.x & 15] = s;
+    __syncthreads();
+    if (lane == 0) {
+        float sum = 0.0f;
+        for (int r = 0; r < 16; ++r) sum = sum + part[r][threadIdx.x];
+        if (column < dim)
+            dq_weight[column] = sum;
+        else
+            dk_weight[column - dim] = sum;
+    }
+}
+
+struct NormCall {
+    const void *const *bufs;
+    int world;
+    void *out[3];
+    const void *grad[3];
+    const void *weight[2];
+    const int64_t *positions;
+    const double *inv_freq;
+    float *partial;
+    size_t tokens;
+    int heads[3];
+    int dim, rotary, interleaved;
+    float eps;
+    bool backward;
+    unsigned workgroups;
+    int tokens_per_wg;
+};
+
+template <class Row, int LANES, int NSRC>
+static hipError_t launch_norm(const NormCall &c, hipStream_t stream)
+{
+    NormArgs<NSRC> a = {};
+    for (int i = 0; i < NSRC; ++i) a.src[i] = static_cast<const char *>(c.bufs[i]);
+    for (int i = 0; i < 3; ++i) {
+        a.out[i] = static_cast<char *>(c.out[i]);
+        a.grad[i] = static_cast<const char *>(c.grad[i]);
+        a.heads[i] = c.heads[i];
+    }
+    for (int i = 0; i < 2; ++i) a.weight[i] = static_cast<const char *>(c.weight[i]);
+    a.positions = c.positions;
+    a.inv_freq = c.inv_freq;
+    a.partial = c.partial;
+    a.tokens = c.tokens;
+    a.rotary = c.rotary;
+    a.interleaved = c.interleaved;
+    a.tokens_per_wg = c.tokens_per_wg;
+    a.eps = c.eps;
+    if (c.backward)
+        hipLaunchKernelGGL((qk_norm_rope_backward_kernel<Row, LANES, NSRC>), dim3(c.workgroups), dim3(kNormBlock), 0,
+                           stream, a);
+    else
+        hipLaunchKernelGGL((qk_norm_rope_kernel<Row, LANES, NSRC>), dim3(c.workgroups), dim3(kNormBlock), 0, stream,
+                           a);
+    return hipGetLastError();
+}
+
+template <class Row, int LANES>
+static hipError_t launch_norm_nsrc(const NormCall &c, hipStream_t stream)
+{
+    switch (c.world) {
+    case 1: return launch_norm<Row, LANES, 1>(c, stream);
+    case 2: return launch_norm<Row, LANES, 2>(c, stream);
+    case 3: return launch_norm<Row, LANES, 3>(c, stream);
+    case 4: return launch_norm<Row, LANES, 4>(c, stream);
+    case 5: return launch_norm<Row, LANES, 5>(c, stream);
+    case 6: return launch_norm<Row, LANES, 6>(c, stream);
+    case 7: return launch_norm<Row, LANES, 7>(c, stream);
+    case 8: return launch_norm<Row, LANES, 8>(c, stream);
+    default: return hipErrorInvalidValue;
+    }
+}
+
+template <class Row>
+static hipError_t launch_norm_dim(const NormCall &c, hipStream_t stream)
+{
+    switch (c.dim) {
+    case 64: return launch_norm_nsrc<Row, 8>(c, stream);
+    case 128: return launch_norm_nsrc<Row, 16>(c, stream);
+    case 256: return launch_norm_nsrc<Row, 32>(c, stream);
+    default: return hipErrorInvalidValue;
+    }
+}
+
+// Tokens a workgroup takes at once: where a token has fewer than four waves' worth of heads, more tokens.
+static int norm_tokens_per_wg(const NormCall &c)
+{
+    const int per_wave = 512 / c.dim;
+    const int groups = (c.heads[0] + c.heads[1] + c.heads[2] + per_wave - 1) / per_wave;
+    return groups >= kNormWaves ? 1 : (groups >= 2 ? 2 : 4);
+}
+
+// Workgroups of the backward pass: each leaves one partial row.
+static unsigned backward_workgroups(const NormCall &c)
+{
+    const size_t need = (c.tokens + c.tokens_per_wg - 1) / c.tokens_per_wg;
+    const size_t most = static_cast<size_t>(compute_units()) * 4;
+    return static_cast<unsigned>(need < most ? need : most);
+}
+
+static int check_norm(const NormCall &c, int dtype)
+{
+    if (c.bufs == nullptr || c.world < 1 || c.world > TCCL_MAX_WORLD) return TCCL_EINVAL;
+    if (dtype != TCCL_BF16 && dtype != TCCL_F32) return TCCL_EINVAL;
+    if (c.dim != 64 && c.dim != 128 && c.dim != 256) return TCCL_EINVAL;
+    if (c.heads[0] < 0 || c.heads[1] < 0 || c.heads[2] < 0) return TCCL_EINVAL;
+    const int64_t all = static_cast<int64_t>(c.heads[0]) + c.heads[1] + c.heads[2];
+    if (all < 1 || all > (1 << 20)) return TCCL_EINVAL;
+    if (c.rotary < 0 || c.rotary > c.dim || c.rotary % 16 != 0) return TCCL_EINVAL;
+    if (!(c.eps >= 0.0f)) return TCCL_EINVAL;
+    if (c.weight[0] == nullptr || c.weight[1] == nullptr || c.positions == nullptr) return TCCL_EINVAL;
+    if (c.rotary > 0 && c.inv_freq == nullptr) return TCCL_EINVAL;
+    if (c.tokens > (static_cast<size_t>(1) << 31) - 1) return TCCL_EINVAL; // one workgroup per token at most
+    if (!aligned16(c.weight[0]) || !aligned16(c.weight[1])) return TCCL_EALIGN;
+    for (int i = 0; i < c.world; ++i) {
+        if (c.bufs[i] == nullptr) return TCCL_EINVAL;
+        if (!aligned16(c.bufs[i])) return TCCL_EALIGN;
+    }
+    for (int i = 0; i < 3; ++i) {
+        if (c.heads[i] > 0 && ((c.backward ? c.grad[i] : c.out[i]) == nullptr)) return TCCL_EINVAL;
+        if (!aligned16(c.grad[i]) || !aligned16(c.out[i])) return TCCL_EALIGN;
+    }
+    return TCCL_OK;
+}
+
+} // namespace tccl
+
+using namespace tccl;
+
+extern "C" int tccl_qk_norm_rope(const void *const *bufs, int world, void *q_out, void *k_out, void *v_out,
+                                 const void *q_weight, const void *k_weight, const int64_t *positions,
+                                 const double *inv_freq, size_t tokens, int q_heads, int k_heads, int v_heads,
+                                 int head_dim, int rotary_dim, int interleaved, float eps, int dtype, void *stream)
+{
+    NormCall c = {};
+    c.bufs = bufs;
+    c.world = world;
+    c.out[0] = q_out, c.out[1] = k_out, c.out[2] = v_out;
+    c.weight[0] = q_weight, c.weight[1] = k_weight;
+    c.positions = positions;
+    c.inv_freq = inv_freq;
+    c.tokens = tokens;
+    c.heads[0] = q_heads, c.heads[1] = k_heads, c.heads[2] = v_heads;
+    c.dim = head_dim, c.rotary = rotary_dim, c.interleaved = interleaved;
+    c.eps = eps;
+    if (const int rc = check_norm(c, dtype)) return rc;
+    if (tokens == 0) return TCCL_OK;
+    c.tokens_per_wg = norm_tokens_per_wg(c);
+    c.workgroups = static_cast<unsigned>((tokens + c.tokens_per_wg - 1) / c.tokens_per_wg);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    return hip_code(dtype == TCCL_BF16 ? launch_norm_dim<Bf16Row>(c, s) : launch_norm_dim<F32Row>(c, s));
+}
+
+extern "C" size_t tccl_qk_norm_rope_backward_workspace(int head_dim)
+{
+    if (head_dim != 64 && head_dim != 128 && head_dim != 256) return 0;
+    return static_cast<size_t>(compute_units()) * 4 * 2 * head_dim * sizeof(float);
+}
+
+extern "C" int tccl_qk_norm_rope_backward(const void *const *bufs, int world, const void *dq, const void *dk,
+                                          const void *dv, const void *q_weight, const void *k_weight,
+                                          const int64_t *positions, const double *inv_freq, void *dx,
+                                          float *dq_weight, float *dk_weight, void *workspace, size_t workspace_bytes,
+                                          size_t tokens, int q_heads, int k_heads, int v_heads, int head_dim,
+                                          int rotary_dim, int interleaved, float eps, int dtype, void *stream)
+{
+    NormCall c = {};
+    c.backward = true;
+    c.bufs = bufs;
+    c.world = world;
+    c.out[0] = dx;
+    c.grad[0] = dq, c.grad[1] = dk, c.grad[2] = dv;
+    c.weight[0] = q_weight, c.weight[1] = k_weight;
+    c.positions = positions;
+    c.inv_freq = inv_freq;
+    c.partial = static_cast<float *>(workspace);
+    c.tokens = tokens;
+    c.heads[0] = q_heads, c.heads[1] = k_heads, c.heads[2] = v_heads;
+    c.dim = head_dim, c.rotary = rotary_dim, c.interleaved = interleaved;
+    c.eps = eps;
+    if (const int rc = check_norm(c, dtype)) return rc;
+    if (dx == nullptr || dq_weight == nullptr || dk_weight == nullptr || workspace == nullptr) return TCCL_EINVAL;
+    if (!aligned16(dq_weight) || !aligned16(dk_weight) || !aligned16(workspace)) return TCCL_EALIGN;
+    if (workspace_bytes < tccl_qk_norm_rope_backward_workspace(head_dim)) return TCCL_ESCRATCH;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (tokens > 0) {
+        c.tokens_per_wg = norm_tokens_per_wg(c);
+        c.workgroups = backward_workgroups(c);
+        const hipError_t e = dtype == TCCL_BF16 ? launch_norm_dim<Bf16Row>(c, s) : launch_norm_dim<F32Row>(c, s);
+        if (e != hipSuccess) return hip_code(e);
+    }
+    // no tokens: no partial rows, and the weight gradients are zero
+    hipLaunchKernelGGL(weight_grad_kernel, dim3(2 * head_dim / 16), dim3(256), 0, s, c.partial,
+                       static_cast<int>(c.workgroups), head_dim, dq_weight, dk_weight);
+    return hip_code(hipGetLastError());
+}
