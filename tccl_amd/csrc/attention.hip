@@ -22,8 +22,8 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kAttnBlock = 256;
 constexpr int kAttnWaves = 4;
-constexpr int kMaxChunk = 8192;  // tokens of a workgroup: 512 pages of 16
-constexpr int kChunkStep = 256;  // chunks are whole pages of every size
+constexpr int kPiecePages = 512;  // page addresses a workgroup looks up at once
+constexpr int kSharedBatch = 4096; // most sequences whose tokens are dealt out evenly
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
 struct AttnArgs {
@@ -35,9 +35,12 @@ struct AttnArgs {
     const int32_t *lengths;
     char *out;
     float *lse;             // may be nullptr
-    float *part_o, *part_ml; // [batch][q_heads][splits][D] and [batch][q_heads][splits][2]
-    int q_heads, group, head_blocks; // query heads, per key head, and blocks of 16 of the latter
-    int most, chunk, splits; // tokens: of a sequence at most, of a workgroup; chunks of `most`
+    float *part_o, *part_ml; // [workgroups][2][heads of a workgroup][D] and [..][2]: see decode_attention_kernel
+    int2 *spans;            // [batch * head_groups]: a row's first partial and how many workgroups it spans
+    int batch, q_heads, group; // query heads: all, and per key head
+    int blocks_per_wg, head_groups; // blocks of 16 query heads in a workgroup (1, 2, 4); rows per sequence
+    int most;               // tokens of a sequence at most
+    int workgroups;         // that share the tokens; 0: a workgroup per row
     float scale;            // times log2(e)
 };
 
@@ -65,6 +68,51 @@ __device__ __forceinline__ int sequence_length(const AttnArgs &a, int b)
     return n < 0 ? 0 : (n < a.most ? n : a.most);
 }
 
+// Dealing out `units` to `workgroups`: the first `rest` of them get one more than the others.
+struct Shares {
+    uint32_t each, rest;
+    __device__ __forceinline__ Shares(uint32_t units, uint32_t workgroups)
+        : each(units / workgroups), rest(units - each * workgroups)
+    {
+    }
+    __device__ __forceinline__ uint32_t begin(uint32_t w) const { return w * each + (w < rest ? w : rest); }
+    __device__ __forceinline__ uint32_t owner(uint32_t unit) const
+    {
+        const uint32_t longer = rest * (each + 1);
+        return unit < longer ? unit / (each + 1) : rest + (unit - longer) / each;
+    }
+};
+
+// Exclusive prefix sum over the workgroup's threads; `total` is the sum.
+__device__ __forceinline__ uint32_t prefix_sum(uint32_t x, uint32_t *wave_sums, uint32_t &total)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t sum = x;
+#pragma unroll
+    for (int step = 1; step < 64; step *= 2) {
+        const uint32_t up = __shfl_up(sum, step);
+        sum += lane >= step ? up : 0;
+    }
+    if (lane == 63) wave_sums[wave] = sum;
+    __syncthreads();
+    uint32_t before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kAttnWaves; ++w) {
+        before += w < wave ? wave_sums[w] : 0;
+        total += wave_sums[w];
+    }
+    return before + sum - x;
+}
+
+// A row is a sequence, a key head and up to 64 of the query heads that share it (blocks of 16); its tokens are
+// cut into units of four token blocks.  All rows' units, one row behind the other, are dealt out evenly to the
+// workgroups, so that ragged lengths leave no workgroup with more than its share.  A row that lies in one
+// workgroup is finished there.  Of the others each workgroup leaves its part of (m, l, O): in place 0 the row
+// that holds its first unit, in place 1 the row that it begins and does not end; join_parts_kernel
+// joins them.  Four waves: blocks_per_wg of them work on different blocks of query heads and the same
+// tokens (which they share through the caches), the others on different tokens.
+//
 // Lane layout, lane = 16 g + m:
 //   K operand    row m is a token, the lane's 16 bytes are its dims 16-byte chunk g of four
 //   Q operand    column m is a query head, the same dims
@@ -74,254 +122,369 @@ __device__ __forceinline__ int sequence_length(const AttnArgs &a, int b)
 // A block is four groups of TOKENS = 8 (bf16) or 16 (8 bits) consecutive tokens.  Row 4 g + i of the block's
 // K tile t is token TOKENS g + 4 t + i, so that S^T leaves the tokens of group g in lanes 16 g ... 16 g + 15,
 // where P^T needs them.
-template <class Store, int D>
-__global__ void __launch_bounds__(kAttnBlock)
+template <class Store, int D, bool NT>
+__global__ void __launch_bounds__(kAttnBlock, D == 256 ? 1 : 2)
 decode_attention_kernel(AttnArgs a)
 {
-    constexpr int TOKENS = Store::kChunk, TILES = TOKENS / 4, BLOCK = 4 * TOKENS;
+    constexpr int TOKENS = Store::kChunk, TILES = TOKENS / 4, BLOCK = 4 * TOKENS, UNIT = kAttnWaves * BLOCK;
     constexpr int KLOADS = D / (4 * Store::kChunk);          // 16-byte chunks of a token's row per lane
     constexpr int QSTEPS = D / 32, DTILES = D / 16, PARTS = TOKENS / 8;
-    __shared__ const char *pages[kMaxChunk / 16];
+    __shared__ const char *pages[kPiecePages];
     __shared__ float wave_m[kAttnWaves][16], wave_l[kAttnWaves][16];
     __shared__ float wave_o[kAttnWaves][16][D + 4];
+    __shared__ uint32_t wave_sums[kAttnWaves], found[3];
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, m = lane & 15;
-    // blockIdx.x = ((b * heads + h) * head_blocks + hb) * splits + split
-    uint32_t rest = blockIdx.x;
-    const int split = rest % a.splits;
-    rest /= a.splits;
-    const int hb = rest % a.head_blocks;
-    rest /= a.head_blocks;
-    const int h = rest % a.shape.heads, b = rest / a.shape.heads;
-    const int length = sequence_length(a, b);
-    const int begin = split * a.chunk;
-    const int in_block = a.group - 16 * hb < 16 ? a.group - 16 * hb : 16; // query heads here
-    const int first_head = h * a.group + 16 * hb;
-    if (begin >= length && split > 0) return;
-    const int end = begin + a.chunk < length ? begin + a.chunk : length;
-    const int count = end - begin; // tokens; 0 only where the sequence is empty
-
     const int shift = a.shape.page_shift, page_size = 1 << shift;
-    const int npages = (count + page_size - 1) >> shift;
-    for (int i = threadIdx.x; i < npages; i += kAttnBlock)
-        pages[i] = a.shape.block(a.table[static_cast<size_t>(b) * a.table_row + (begin >> shift) + i], h);
-
-    u32x4 q[QSTEPS];
-#pragma unroll
-    for (int s = 0; s < QSTEPS; ++s) {
-        // the dims of contraction step s that lane group g holds
-        const int dim = Store::kScaled ? (s >> 1) * 64 + g * 16 + (s & 1) * 8 : s * 32 + g * 8;
-        q[s] = u32x4{0, 0, 0, 0};
-        if (m < in_block)
-            q[s] = load_vec<false>(a.q + b * a.q_batch + (first_head + m) * a.q_head + dim * 2, 0);
-    }
-    __syncthreads();
-
     const size_t v_at = static_cast<size_t>(page_size) * D * Store::kBytes;
     const char *const safe = a.shape.pool.p[0]; // read, and masked, where there is no page
-    float top = -__builtin_inff(), total = 0.0f;
-    f32x4 acc[DTILES];
-#pragma unroll
-    for (int i = 0; i < DTILES; ++i) acc[i] = f32x4{0, 0, 0, 0};
+    const int my_block = wave % a.blocks_per_wg, my_turn = wave / a.blocks_per_wg, turns = kAttnWaves / a.blocks_per_wg;
 
-    for (int start = wave * BLOCK; start < count; start += kAttnWaves * BLOCK) {
-        // keys: lane m's token of tile t lies in group m / 4; values and scores: group g
-        const int kt = start + (m >> 2) * TOKENS, vt = start + g * TOKENS;
-        const int kp = kt >> shift, vp = vt >> shift;
-        const char *kb = kp < npages ? pages[kp] : nullptr;
-        const char *vb = vp < npages ? pages[vp] : nullptr;
-        int live = vb != nullptr ? count - vt : 0; // tokens of group g that count
-        live = live < 0 ? 0 : live;
-        kb = kb != nullptr ? kb : safe;
-        vb = vb != nullptr ? vb : safe;
-        const int ko = kt & (page_size - 1), vo = vt & (page_size - 1);
-        u32x4 k[TILES][KLOADS], v[DTILES];
+    // the workgroup's units [unit, stop) of all, and the row that `unit` lies in
+    uint32_t unit, stop, row_begin; // row_begin: the first unit of the row
+    int b, hg, length;
+    Shares shares(0, 1);
+    if (a.workgroups == 0) {
+        b = blockIdx.x / a.head_groups;
+        hg = blockIdx.x % a.head_groups;
+        length = sequence_length(a, b);
+        unit = row_begin = 0;
+        stop = (length + UNIT - 1) / UNIT;
+        if (length == 0) stop = 1; // an empty row: one pass over no tokens, which writes its zeros
+    } else {
+        const int per = (a.batch + kAttnBlock - 1) / kAttnBlock, first = threadIdx.x * per;
+        const int last = first + per < a.batch ? first + per : a.batch;
+        uint32_t mine = 0;
+        for (int i = first; i < last; ++i) mine += (sequence_length(a, i) + UNIT - 1) / UNIT;
+        uint32_t all;
+        uint32_t before = prefix_sum(mine, wave_sums, all);
+        shares = Shares(all * a.head_groups, gridDim.x);
+        unit = shares.begin(blockIdx.x);
+        stop = shares.begin(blockIdx.x + 1);
+        if (unit < stop && unit >= before * a.head_groups && unit < (before + mine) * a.head_groups) {
+            for (int i = first; i < last; ++i) {
+                const int n = sequence_length(a, i);
+                const uint32_t units = (n + UNIT - 1) / UNIT;
+                if (unit < (before + units) * a.head_groups) {
+                    found[0] = i;
+                    found[1] = before * a.head_groups;
+                    found[2] = n;
+                    break;
+                }
+                before += units;
+            }
+        }
+        // rows without tokens have no units: their zeros are written here
+        for (int e = blockIdx.x; e < a.batch; e += gridDim.x) {
+            if (sequence_length(a, e) > 0) continue;
+            const size_t row = static_cast<size_t>(e) * a.q_heads;
+            for (int i = threadIdx.x; i < a.q_heads * (D / 8); i += kAttnBlock)
+                store_vec<false>(a.out + row * D * 2, i, u32x4{0, 0, 0, 0});
+            for (int i = threadIdx.x; i < a.q_heads; i += kAttnBlock)
+                if (a.lse != nullptr) a.lse[row + i] = -__builtin_inff();
+            for (int i = threadIdx.x; i < a.head_groups; i += kAttnBlock) a.spans[e * a.head_groups + i] = int2{0, 0};
+        }
+        if (unit == stop) return;
+        __syncthreads();
+        b = found[0];
+        length = found[2];
+        const uint32_t n = (length + UNIT - 1) / UNIT;
+        hg = (unit - found[1]) / n;
+        row_begin = found[1] + hg * n;
+    }
+
+    for (bool first_row = true; unit < stop; first_row = false) {
+        const uint32_t row_units = length == 0 ? 1 : (length + UNIT - 1) / UNIT;
+        const uint32_t row_end = row_begin + row_units, until = row_end < stop ? row_end : stop;
+        const int groups_per_head = a.head_groups / a.shape.heads;
+        const int h = hg / groups_per_head, first_of_group = hg % groups_per_head * a.blocks_per_wg * 16;
+        const int left = a.group - first_of_group, in_wg = left < 16 * a.blocks_per_wg ? left : 16 * a.blocks_per_wg;
+        const int first_head = h * a.group + first_of_group; // of the workgroup's in_wg query heads
+        const int in_block = in_wg - 16 * my_block;          // of the wave's, may be over 16 or below 1
+
+        u32x4 q[QSTEPS];
 #pragma unroll
-        for (int t = 0; t < TILES; ++t) {
-            const int at = ko + 4 * t + (m & 3);
-            const char *row = kb + static_cast<size_t>(at >> 4) * (D / Store::kChunk) * 256 + (at & 15) * 16;
+        for (int s = 0; s < QSTEPS; ++s) {
+            // the dims of contraction step s that lane group g holds
+            const int dim = Store::kScaled ? (s >> 1) * 64 + g * 16 + (s & 1) * 8 : s * 32 + g * 8;
+            q[s] = u32x4{0, 0, 0, 0};
+            if (m < in_block)
+                q[s] = load_vec<false>(
+                    a.q + b * a.q_batch + (first_head + 16 * my_block + m) * a.q_head + dim * 2, 0);
+        }
+        float top = -__builtin_inff(), total = 0.0f;
+        f32x4 acc[DTILES];
 #pragma unroll
-            for (int c = 0; c < KLOADS; ++c) k[t][c] = load_vec<false>(row + (c * 4 + g) * 256, 0);
+        for (int i = 0; i < DTILES; ++i) acc[i] = f32x4{0, 0, 0, 0};
+
+        const int row_stop = static_cast<int>(until - row_begin) * UNIT < length
+                                 ? static_cast<int>(until - row_begin) * UNIT
+                                 : length;
+        for (int begin = static_cast<int>(unit - row_begin) * UNIT; begin < row_stop;) {
+            // a piece: what kPiecePages pages cover, in whole units
+            const int first_page = begin >> shift;
+            const int reach = ((first_page + kPiecePages) << shift) / UNIT * UNIT;
+            const int end = reach < row_stop && reach > 0 ? reach : row_stop;
+            const int npages = ((end - 1) >> shift) - first_page + 1;
+            __syncthreads();
+            for (int i = threadIdx.x; i < npages; i += kAttnBlock)
+                pages[i] = a.shape.block(a.table[static_cast<size_t>(b) * a.table_row + first_page + i], h);
+            __syncthreads();
+
+            u32x4 k[TILES][KLOADS], v[DTILES], k_scales = {}, v_scales = {};
+            // lane m's token of tile t lies in group m / 4 of the block
+            auto load_keys = [&](int start) {
+                const int at = start + (m >> 2) * TOKENS, p = (at >> shift) - first_page;
+                const char *kb = p < npages ? pages[p] : nullptr;
+                kb = kb != nullptr ? kb : safe;
+#pragma unroll
+                for (int t = 0; t < TILES; ++t) {
+                    const int in = (at & (page_size - 1)) + 4 * t + (m & 3);
+                    const char *row = kb + static_cast<size_t>(in >> 4) * (D / Store::kChunk) * 256 + (in & 15) * 16;
+#pragma unroll
+                    for (int c = 0; c < KLOADS; ++c) k[t][c] = load_vec<NT>(row + (c * 4 + g) * 256, 0);
+                }
+            };
+            // values and scores: group g.  `live`: the tokens of it that count
+            int live = 0;
+            auto load_values = [&](int start) {
+                const int at = start + g * TOKENS, p = (at >> shift) - first_page;
+                const char *vb = p < npages ? pages[p] : nullptr;
+                live = vb != nullptr ? end - at : 0;
+                vb = vb != nullptr ? vb : safe;
+                const int in = at & (page_size - 1);
+#pragma unroll
+                for (int d = 0; d < DTILES; ++d)
+                    v[d] = load_vec<NT>(vb + v_at + (static_cast<size_t>(in / TOKENS) * D + d * 16 + m) * 16, 0);
+                if constexpr (Store::kScaled) {
+                    k_scales = load_vec<false>(vb + 2 * v_at + in, 0);
+                    v_scales = load_vec<false>(vb + 2 * v_at + page_size + in, 0);
+                }
+            };
+            int start = begin + my_turn * BLOCK;
+            if (start < end) {
+                load_keys(start);
+                load_values(start);
+            }
+            for (; start < end; start += turns * BLOCK) {
+                const int next = start + turns * BLOCK;
+                f32x4 s[TILES];
+#pragma unroll
+                for (int t = 0; t < TILES; ++t) s[t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < KLOADS; ++i) // tiles innermost: their chains of products do not wait for each other
+#pragma unroll
+                    for (int half = 0; half < (Store::kScaled ? 2 : 1); ++half)
+#pragma unroll
+                        for (int t = 0; t < TILES; ++t) {
+                            if constexpr (Store::kScaled)
+                                s[t] = mfma(widen_e4m3(k[t][i][2 * half], k[t][i][2 * half + 1]), q[2 * i + half], s[t]);
+                            else
+                                s[t] = mfma(k[t][i], q[i], s[t]);
+                        }
+                if (next < end) load_keys(next);
+#pragma unroll
+                for (int t = 0; t < TILES; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float x = s[t][i] * a.scale;
+                        if constexpr (Store::kScaled) x = x * scale_of((k_scales[t] >> (8 * i)) & 0xFFu);
+                        s[t][i] = 4 * t + i < live ? x : -__builtin_inff();
+                    }
+                float best = s[0][0];
+#pragma unroll
+                for (int t = 0; t < TILES; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) best = fmaxf(best, s[t][i]);
+                best = across32<MaxOp>(across16<MaxOp>(best));
+                if (__any(best > top)) {
+                    const float higher = fmaxf(top, best);
+                    const float f = higher == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(top - higher);
+                    top = higher;
+                    total = total * f;
+#pragma unroll
+                    for (int d = 0; d < DTILES; ++d) acc[d] = acc[d] * f;
+                }
+                const float from = top == -__builtin_inff() ? 0.0f : top;
+#pragma unroll
+                for (int t = 0; t < TILES; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float p = __builtin_amdgcn_exp2f(s[t][i] - from);
+                        total = total + p;
+                        s[t][i] = p;
+                        if constexpr (Store::kScaled)
+                            s[t][i] = 4 * t + i < live ? p * scale_of((v_scales[t] >> (8 * i)) & 0xFFu) : 0.0f;
+                    }
+                if (!__all(live >= TOKENS)) { // what lies behind the last token may be anything, NaN too
+                    constexpr int EACH = 4 / Store::kBytes;
+#pragma unroll
+                    for (int d = 0; d < DTILES; ++d)
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            const int in_word = live - w * EACH;
+                            v[d][w] &= in_word >= EACH ? ~0u
+                                                       : (in_word <= 0 ? 0u : (1u << (8 * Store::kBytes * in_word)) - 1u);
+                        }
+                }
+#pragma unroll
+                for (int part = 0; part < PARTS; ++part) {
+                    // P in two bf16 terms, so that its rounding (2^-9 of each weight) does not reach the output
+                    u32x4 hi, lo;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const float x = s[2 * part + (w >> 1)][(2 * w) & 3], y = s[2 * part + (w >> 1)][(2 * w + 1) & 3];
+                        hi[w] = pack_bf16(x, y);
+                        lo[w] = pack_bf16(x - bits_to_f32(hi[w] << 16), y - bits_to_f32(hi[w] & 0xFFFF0000u));
+                    }
+#pragma unroll
+                    for (int d = 0; d < DTILES; ++d) {
+                        u32x4 vd;
+                        if constexpr (Store::kScaled)
+                            vd = widen_e4m3(v[d][2 * part], v[d][2 * part + 1]);
+                        else
+                            vd = v[d];
+                        acc[d] = mfma(vd, hi, acc[d]);
+                        acc[d] = mfma(vd, lo, acc[d]);
+                    }
+                }
+                if (next < end) load_values(next);
+            }
+            begin = end;
+        }
+
+        // the waves' parts: lane groups hold the sums of their own tokens, and all dims of O
+        total = across32<AddOp>(across16<AddOp>(total));
+        __syncthreads();
+        if (g == 0) {
+            wave_m[wave][m] = top;
+            wave_l[wave][m] = total;
         }
 #pragma unroll
         for (int d = 0; d < DTILES; ++d)
-            v[d] = load_vec<false>(vb + v_at + (static_cast<size_t>(vo / TOKENS) * D + d * 16 + m) * 16, 0);
-        float s[TILES][4], pv[TILES][4];
-        u32x4 k_scales, v_scales;
-        if constexpr (Store::kScaled) {
-            k_scales = load_vec<false>(vb + 2 * v_at + vo, 0);
-            v_scales = load_vec<false>(vb + 2 * v_at + page_size + vo, 0);
-        }
 #pragma unroll
-        for (int t = 0; t < TILES; ++t) {
-            f32x4 c = {0, 0, 0, 0};
+            for (int i = 0; i < 4; ++i) wave_o[wave][m][d * 16 + 4 * g + i] = acc[d][i];
+        __syncthreads();
+        const bool whole = unit == row_begin && until == row_end;
+        const size_t part = 2 * blockIdx.x + (first_row ? 0 : 1);
+        for (int item = threadIdx.x; item < in_wg * (D / 4); item += kAttnBlock) {
+            const int n = item / (D / 4), d = item % (D / 4) * 4, block = n >> 4, at = n & 15;
+            float best = -__builtin_inff();
+            for (int w = block; w < kAttnWaves; w += a.blocks_per_wg) best = fmaxf(best, wave_m[w][at]);
+            const float from = best == -__builtin_inff() ? 0.0f : best;
+            float l = 0.0f;
+            f32x4 o = {0, 0, 0, 0};
+            for (int w = block; w < kAttnWaves; w += a.blocks_per_wg) {
+                const float f = __builtin_amdgcn_exp2f(wave_m[w][at] - from);
+                l = __builtin_fmaf(wave_l[w][at], f, l);
 #pragma unroll
-            for (int i = 0; i < KLOADS; ++i) {
-                if constexpr (Store::kScaled) {
-                    c = mfma(widen_e4m3(k[t][i][0], k[t][i][1]), q[2 * i], c);
-                    c = mfma(widen_e4m3(k[t][i][2], k[t][i][3]), q[2 * i + 1], c);
-                } else {
-                    c = mfma(k[t][i], q[i], c);
+                for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(wave_o[w][at][d + i], f, o[i]);
+            }
+            if (whole) {
+                const size_t row = static_cast<size_t>(b) * a.q_heads + first_head + n;
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                *reinterpret_cast<u32x2 *>(a.out + (row * D + d) * 2) =
+                    u32x2{pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv)};
+                if (d == 0 && a.lse != nullptr)
+                    a.lse[row] = l == 0.0f ? -__builtin_inff() : (best + __builtin_amdgcn_logf(l)) * kLn2;
+            } else {
+                const size_t to = part * (16 * a.blocks_per_wg) + n;
+                *reinterpret_cast<f32x4 *>(a.part_o + to * D + d) = o;
+                if (d == 0) {
+                    a.part_ml[2 * to] = best;
+                    a.part_ml[2 * to + 1] = l;
                 }
             }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float x = c[i] * a.scale;
-                if constexpr (Store::kScaled) x = x * scale_of((k_scales[t] >> (8 * i)) & 0xFFu);
-                s[t][i] = 4 * t + i < live ? x : -__builtin_inff();
-            }
         }
-        float best = s[0][0];
-#pragma unroll
-        for (int t = 0; t < TILES; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) best = fmaxf(best, s[t][i]);
-        best = across32<MaxOp>(across16<MaxOp>(best));
-        if (__any(best > top)) {
-            const float next = fmaxf(top, best);
-            const float f = next == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(top - next);
-            top = next;
-            total = total * f;
-#pragma unroll
-            for (int d = 0; d < DTILES; ++d) acc[d] = acc[d] * f;
-        }
-        const float from = top == -__builtin_inff() ? 0.0f : top;
-#pragma unroll
-        for (int t = 0; t < TILES; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float p = __builtin_amdgcn_exp2f(s[t][i] - from);
-                total = total + p;
-                pv[t][i] = p;
-                if constexpr (Store::kScaled)
-                    pv[t][i] = 4 * t + i < live ? p * scale_of((v_scales[t] >> (8 * i)) & 0xFFu) : 0.0f;
-            }
-        if (!__all(live >= TOKENS)) { // what lies behind the last token may be anything, NaN too
-#pragma unroll
-            for (int d = 0; d < DTILES; ++d)
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    constexpr int EACH = 4 / Store::kBytes;
-                    const int in_word = live - w * EACH;
-                    const uint32_t keep = in_word >= EACH ? ~0u : (in_word <= 0 ? 0u : (1u << (8 * Store::kBytes * in_word)) - 1u);
-                    v[d][w] &= keep;
-                }
-        }
-#pragma unroll
-        for (int part = 0; part < PARTS; ++part) {
-            // P in two bf16 terms, so that its rounding (2^-9 of each weight) does not reach the output
-            u32x4 hi, lo;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const float x = pv[2 * part + (w >> 1)][(2 * w) & 3], y = pv[2 * part + (w >> 1)][(2 * w + 1) & 3];
-                hi[w] = pack_bf16(x, y);
-                lo[w] = pack_bf16(x - bits_to_f32(hi[w] << 16), y - bits_to_f32(hi[w] & 0xFFFF0000u));
-            }
-#pragma unroll
-            for (int d = 0; d < DTILES; ++d) {
-                u32x4 vd;
-                if constexpr (Store::kScaled)
-                    vd = widen_e4m3(v[d][2 * part], v[d][2 * part + 1]);
-                else
-                    vd = v[d];
-                acc[d] = mfma(vd, hi, acc[d]);
-                acc[d] = mfma(vd, lo, acc[d]);
-            }
-        }
-    }
-
-    // the four waves' parts: lane groups hold the sums of their own tokens, and all dims of O
-    total = across32<AddOp>(across16<AddOp>(total));
-    if (g == 0) {
-        wave_m[wave][m] = top;
-        wave_l[wave][m] = total;
-    }
-#pragma unroll
-    for (int d = 0; d < DTILES; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) wave_o[wave][m][d * 16 + 4 * g + i] = acc[d][i];
-    __syncthreads();
-    const bool whole = a.splits == 1;
-    for (int item = threadIdx.x; item < in_block * (D / 4); item += kAttnBlock) {
-        const int n = item / (D / 4), d = item % (D / 4) * 4;
-        float best = wave_m[0][n];
-#pragma unroll
-        for (int w = 1; w < kAttnWaves; ++w) best = fmaxf(best, wave_m[w][n]);
-        const float from = best == -__builtin_inff() ? 0.0f : best;
-        float l = 0.0f;
-        f32x4 o = {0, 0, 0, 0};
-#pragma unroll
-        for (int w = 0; w < kAttnWaves; ++w) {
-            const float f = __builtin_amdgcn_exp2f(wave_m[w][n] - from);
-            l = __builtin_fmaf(wave_l[w][n], f, l);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(wave_o[w][n][d + i], f, o[i]);
-        }
-        const size_t row = static_cast<size_t>(b) * a.q_heads + first_head + n;
-        if (whole) {
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            *reinterpret_cast<u32x2 *>(a.out + (row * D + d) * 2) =
-                u32x2{pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv)};
-            if (d == 0 && a.lse != nullptr)
-                a.lse[row] = l == 0.0f ? -__builtin_inff() : (best + __builtin_amdgcn_logf(l)) * kLn2;
-        } else {
-            const size_t at = row * a.splits + split;
-            *reinterpret_cast<f32x4 *>(a.part_o + at * D + d) = o;
-            if (d == 0) {
-                a.part_ml[2 * at] = best;
-                a.part_ml[2 * at + 1] = l;
-            }
+        if (a.workgroups == 0) return;
+        if (unit == row_begin && threadIdx.x == 0)
+            a.spans[b * a.head_groups + hg] =
+                int2{static_cast<int>(part), static_cast<int>(shares.owner(row_end - 1) - blockIdx.x) + 1};
+        // the next row
+        unit = until;
+        row_begin = row_end;
+        if (++hg == a.head_groups) {
+            hg = 0;
+            if (unit < stop)
+                do length = sequence_length(a, ++b);
+                while (length == 0);
         }
     }
 }
 
-// One workgroup per (sequence, query head): D / 4 lanes of four dims, the others take every n-th chunk.
-template <int D>
+// WAVES waves per (sequence, query head) that spans several workgroups.  Each lane weighs one part of 64 at a
+// time (every wave all of them), then a wave adds its parts up, D / 64 dims per lane, with sixteen parts' loads in
+// flight; a part's weight reaches the other lanes through a scalar register.
+template <int D, int WAVES>
 __global__ void __launch_bounds__(256)
-join_chunks_kernel(AttnArgs a)
+join_parts_kernel(AttnArgs a)
 {
-    constexpr int LANES = D / 4, ROWS = 256 / LANES;
-    __shared__ float part[ROWS][D + 2];
-    const size_t row = blockIdx.x;
-    const int length = sequence_length(a, static_cast<int>(row / a.q_heads));
-    const int live = length == 0 ? 1 : (length + a.chunk - 1) / a.chunk;
-    const int d = threadIdx.x % LANES * 4, r = threadIdx.x / LANES;
-    const float *const ml = a.part_ml + row * a.splits * 2;
-    const float *const po = a.part_o + row * a.splits * D;
+    constexpr int EACH = D / 64, FLIGHT = 16;
+    typedef float part_t __attribute__((ext_vector_type(EACH)));
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, mine = WAVES == 1 ? 0 : wave;
+    const int row = WAVES == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
+    if (row >= a.batch * a.q_heads) return;
+    const int b = row / a.q_heads, head = row - b * a.q_heads;
+    const int wide = 16 * a.blocks_per_wg, h = head / a.group, in_group = head - h * a.group;
+    const int hg = h * (a.head_groups / a.shape.heads) + in_group / wide, at = in_group % wide;
+    const int2 span = a.spans[b * a.head_groups + hg];
+    if (span.y <= 1) return;
+    // the first part may be in either place of its workgroup, the others are in place 0 of theirs
+    const size_t first = static_cast<size_t>(span.x) * wide + at, others = static_cast<size_t>(span.x / 2) * 2 * wide + at;
+    auto place = [&](int i) { return i == 0 ? first : others + static_cast<size_t>(2 * wide) * i; };
     float best = -__builtin_inff();
-    for (int i = r; i < live; i += ROWS) best = fmaxf(best, ml[2 * i]);
-    if (d == 0) part[r][0] = best;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i) best = fmaxf(best, part[i][0]);
-    __syncthreads();
+    for (int i = lane; i < span.y; i += 64) best = fmaxf(best, a.part_ml[2 * place(i)]);
+    best = across32<MaxOp>(reduce_row<MaxOp, 32>(best));
     const float from = best == -__builtin_inff() ? 0.0f : best;
-    float l = 0.0f;
-    f32x4 o = {0, 0, 0, 0};
-    for (int i = r; i < live; i += ROWS) {
-        const float f = __builtin_amdgcn_exp2f(ml[2 * i] - from);
-        const f32x4 x = *reinterpret_cast<const f32x4 *>(po + static_cast<size_t>(i) * D + d);
-        l = __builtin_fmaf(ml[2 * i + 1], f, l);
+    float l = 0.0f, o[EACH] = {};
+    for (int base = 0; base < span.y; base += 64) {
+        const int here = span.y - base < 64 ? span.y - base : 64;
+        float f = 0.0f;
+        if (lane < here) {
+            const size_t p = place(base + lane);
+            f = __builtin_amdgcn_exp2f(a.part_ml[2 * p] - from);
+            l = __builtin_fmaf(a.part_ml[2 * p + 1], f, l);
+        }
+        const int weight = __builtin_bit_cast(int, f);
+        for (int i = mine * FLIGHT; i < here; i += WAVES * FLIGHT) {
+            part_t x[FLIGHT]; // behind the last part the last one again, which is not used
 #pragma unroll
-        for (int k = 0; k < 4; ++k) o[k] = __builtin_fmaf(x[k], f, o[k]);
+            for (int u = 0; u < FLIGHT; ++u) {
+                const int j = i + u < here ? i + u : here - 1;
+                x[u] = reinterpret_cast<const part_t *>(a.part_o + place(base + j) * D)[lane];
+            }
+#pragma unroll
+            for (int u = 0; u < FLIGHT; ++u) {
+                if (i + u >= here) break;
+                const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(weight, i + u));
+#pragma unroll
+                for (int k = 0; k < EACH; ++k) o[k] = __builtin_fmaf(x[u][k], w, o[k]);
+            }
+        }
     }
+    l = across32<AddOp>(reduce_row<AddOp, 32>(l));
+    if constexpr (WAVES > 1) {
+        __shared__ float sums[WAVES][64 * EACH];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) part[r][d + k] = o[k];
-    if (d == 0) part[r][D] = l;
-    __syncthreads();
-    if (r > 0) return;
-    l = 0.0f;
-    o = f32x4{0, 0, 0, 0};
+        for (int k = 0; k < EACH; ++k) sums[wave][k * 64 + lane] = o[k];
+        __syncthreads();
+        if (wave > 0) return;
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-        l = l + part[i][D];
+        for (int k = 0; k < EACH; ++k) {
+            o[k] = sums[0][k * 64 + lane];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) o[k] = o[k] + part[i][d + k];
+            for (int w = 1; w < WAVES; ++w) o[k] = o[k] + sums[w][k * 64 + lane];
+        }
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    *reinterpret_cast<u32x2 *>(a.out + (row * D + d) * 2) =
-        u32x2{pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv)};
-    if (d == 0 && a.lse != nullptr)
+    uint16_t *out = reinterpret_cast<uint16_t *>(a.out) + static_cast<size_t>(row) * D + lane * EACH;
+    if constexpr (EACH == 1)
+        *out = static_cast<uint16_t>(pack_bf16(o[0] * inv, 0.0f));
+    else if constexpr (EACH == 2)
+        *reinterpret_cast<uint32_t *>(out) = pack_bf16(o[0] * inv, o[1] * inv);
+    else
+        *reinterpret_cast<u32x2 *>(out) = u32x2{pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv)};
+    if (lane == 0 && a.lse != nullptr)
         a.lse[row] = l == 0.0f ? -__builtin_inff() : (best + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
@@ -413,48 +576,64 @@ static hipError_t launch_join_nsrc(const void *const *outs, const void *const *l
 // ------------------------------------------------------------------ launch shape
 
 struct AttnPlan {
-    int chunk, splits, head_blocks;
-    size_t workspace;
+    int blocks_per_wg, head_groups, workgroups;
+    size_t part_floats, span_bytes, workspace;
 };
 
-// Chunks such that the launch has about four workgroups per compute unit if every sequence has `most` tokens,
-// in steps of 256 tokens.
+// How many workgroups share the tokens: two per compute unit (one of head_dim 256, whose registers fill it), but
+// no more than there are units.  Measured with 64 sequences of 2,048 to 8,192 tokens in 8 bits, 8 key heads: one 132 us,
+// two 122, three 135; with 3 of 50,000 to 200,000 and one key head of 256: one 97, two 107.  A workgroup per row
+// and no second launch instead
+//   - where no sequence has over 512 tokens: 32 x 500 tokens, 8 key heads 15.4 us against 19.5;
+//   - where the rows alone fill the GPU eight times and none is so long that the last one would be waited for:
+//     512 x 500 tokens 123 us against 163, 256 x 1,000 126 against 133, but 128 x 2,000 136 against 126;
+//   - where dealing out would take too long in each workgroup (over 4,096 sequences).
 static AttnPlan plan_attention(size_t batch, int q_heads, int kv_heads, int head_dim, int most)
 {
-    AttnPlan p;
-    p.head_blocks = (q_heads / kv_heads + 15) / 16;
-    const size_t rows = batch * kv_heads * p.head_blocks;
-    const size_t want = static_cast<size_t>(compute_units()) * 4;
-    size_t splits = rows == 0 ? 1 : (want + rows - 1) / rows;
-    size_t chunk = (static_cast<size_t>(most) + splits - 1) / splits;
-    chunk = (chunk + kChunkStep - 1) / kChunkStep * kChunkStep;
-    chunk = chunk < kChunkStep ? kChunkStep : (chunk > kMaxChunk ? kMaxChunk : chunk);
-    p.chunk = static_cast<int>(chunk);
-    p.splits = most <= 0 ? 1 : static_cast<int>((static_cast<size_t>(most) + chunk - 1) / chunk);
-    p.workspace = p.splits == 1 ? 0 : batch * q_heads * p.splits * (head_dim + 2) * sizeof(float);
+    AttnPlan p = {};
+    const int blocks = (q_heads / kv_heads + 15) / 16;
+    p.blocks_per_wg = blocks >= 3 ? 4 : blocks;
+    p.head_groups = kv_heads * ((blocks + p.blocks_per_wg - 1) / p.blocks_per_wg);
+    const size_t rows = batch * p.head_groups, units = compute_units();
+    const size_t most_units = rows * ((static_cast<size_t>(most) + 127) / 128); // a unit is 128 or 256 tokens
+    if (most <= 512 || (rows >= 8 * units && most <= 2048) || batch > kSharedBatch ||
+        most_units >= (static_cast<size_t>(1) << 31))
+        return p;
+    const size_t at_once = units * (head_dim == 256 ? 1 : 2), wgs = at_once < most_units ? at_once : most_units;
+    p.workgroups = static_cast<int>(wgs);
+    p.part_floats = 2 * wgs * 16 * p.blocks_per_wg * head_dim;
+    p.span_bytes = rows * sizeof(int2);
+    p.workspace = p.part_floats * sizeof(float) + p.part_floats / head_dim * 2 * sizeof(float) + p.span_bytes;
     return p;
 }
 
 template <class Store, int D>
-static hipError_t launch_attention(const AttnArgs &a, size_t batch, hipStream_t stream)
+static hipError_t launch_attention(const AttnArgs &a, hipStream_t stream)
 {
-    const size_t grid = batch * a.shape.heads * a.head_blocks * a.splits;
-    hipLaunchKernelGGL((decode_attention_kernel<Store, D>), dim3(static_cast<unsigned>(grid)), dim3(kAttnBlock), 0,
-                       stream, a);
+    const size_t grid = a.workgroups > 0 ? a.workgroups : static_cast<size_t>(a.batch) * a.head_groups;
+    if (a.blocks_per_wg == 1)
+        hipLaunchKernelGGL((decode_attention_kernel<Store, D, true>), dim3(static_cast<unsigned>(grid)),
+                           dim3(kAttnBlock), 0, stream, a);
+    else
+        hipLaunchKernelGGL((decode_attention_kernel<Store, D, false>), dim3(static_cast<unsigned>(grid)),
+                           dim3(kAttnBlock), 0, stream, a);
     const hipError_t e = hipGetLastError();
-    if (e != hipSuccess || a.splits == 1) return e;
-    hipLaunchKernelGGL((join_chunks_kernel<D>), dim3(static_cast<unsigned>(batch * a.q_heads)), dim3(256), 0, stream,
-                       a);
+    if (e != hipSuccess || a.workgroups == 0) return e;
+    const unsigned rows = static_cast<unsigned>(a.batch) * a.q_heads;
+    if (static_cast<size_t>(a.workgroups) >= 8 * static_cast<size_t>(a.batch) * a.head_groups)
+        hipLaunchKernelGGL((join_parts_kernel<D, 4>), dim3(rows), dim3(256), 0, stream, a);
+    else
+        hipLaunchKernelGGL((join_parts_kernel<D, 1>), dim3((rows + 3) / 4), dim3(256), 0, stream, a);
     return hipGetLastError();
 }
 
 template <class Store>
-static hipError_t launch_attention_dim(const AttnArgs &a, size_t batch, int dim, hipStream_t stream)
+static hipError_t launch_attention_dim(const AttnArgs &a, int dim, hipStream_t stream)
 {
     switch (dim) {
-    case 64: return launch_attention<Store, 64>(a, batch, stream);
-    case 128: return launch_attention<Store, 128>(a, batch, stream);
-    case 256: return launch_attention<Store, 256>(a, batch, stream);
+    case 64: return launch_attention<Store, 64>(a, stream);
+    case 128: return launch_attention<Store, 128>(a, stream);
+    case 256: return launch_attention<Store, 256>(a, stream);
     default: return hipErrorInvalidValue;
     }
 }
@@ -494,27 +673,28 @@ extern "C" int tccl_decode_attention(const tccl_paged_cache *cache, const void *
     if (batch == 0) return TCCL_OK;
     const AttnPlan plan = plan_attention(batch, q_heads, cache->kv_heads, cache->head_dim, max_tokens);
     if (plan.workspace > 0 && (workspace == nullptr || workspace_bytes < plan.workspace)) return TCCL_ESCRATCH;
-    if (batch * cache->kv_heads * plan.head_blocks * plan.splits > 0x7FFFFFFFull || batch * q_heads > 0x7FFFFFFFull)
-        return TCCL_EINVAL;
+    if (batch * plan.head_groups > 0x7FFFFFFFull || batch * q_heads > 0x7FFFFFFFull) return TCCL_EINVAL;
     a.q = static_cast<const char *>(q);
     a.table = page_table;
     a.table_row = page_table_stride;
     a.lengths = lengths;
     a.out = static_cast<char *>(out);
     a.lse = lse;
-    // the maxima and sums lie behind the partial outputs
+    // the workspace: partial outputs, their maxima and sums, the rows' spans
     a.part_o = static_cast<float *>(workspace);
-    a.part_ml = a.part_o + (plan.workspace > 0 ? batch * q_heads * plan.splits * cache->head_dim : 0);
+    a.part_ml = a.part_o + plan.part_floats;
+    a.spans = reinterpret_cast<int2 *>(a.part_ml + plan.part_floats / cache->head_dim * 2);
+    a.batch = static_cast<int>(batch);
     a.q_heads = q_heads;
     a.group = q_heads / cache->kv_heads;
-    a.head_blocks = plan.head_blocks;
+    a.blocks_per_wg = plan.blocks_per_wg;
+    a.head_groups = plan.head_groups;
     a.most = max_tokens;
-    a.chunk = plan.chunk;
-    a.splits = plan.splits;
+    a.workgroups = plan.workgroups;
     a.scale = scale * kLog2e;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    return hip_code(cache->dtype == TCCL_E4M3 ? launch_attention_dim<E4m3Store>(a, batch, cache->head_dim, s)
-                                              : launch_attention_dim<Bf16Store>(a, batch, cache->head_dim, s));
+    return hip_code(cache->dtype == TCCL_E4M3 ? launch_attention_dim<E4m3Store>(a, cache->head_dim, s)
+                                              : launch_attention_dim<Bf16Store>(a, cache->head_dim, s));
 }
 
 extern "C" int tccl_attention_all_reduce(const void *const *outs, const void *const *lses, int world, void *out,

@@ -422,6 +422,11 @@ ATTENTION_CASES = [
     (1, [20011], 4, 2, 64, 16, BF16),
     (7, [20011], 7, 1, 128, 16, E4M3),
     (6, [40, 41] * 40, 3, 3, 64, 16, BF16),
+    (2, [0, 0, 900, 0, 130, 2, 0], 70, 2, 64, 16, BF16),
+    (2, [0, 5, 600, 0, 1300, 2, 0] * 3, 35, 1, 128, 32, E4M3),
+    (1, [530, 0] + [3] * 300, 2, 2, 64, 16, E4M3),
+    (3, [5, 0, 17, 1] * 1100, 1, 1, 64, 16, BF16),
+    (1, [600] + [0, 3] * 2100, 2, 1, 64, 16, BF16),
 ]
 
 
