@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import math
 from typing import Optional, Tuple, Union
 
@@ -30,13 +31,19 @@ PAGE_SIZES = (16, 32, 64, 128, 256)
 _STORES = {torch.bfloat16: _lib.TCCL_BF16, torch.float8_e4m3fn: _lib.TCCL_E4M3}
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(device: torch.device):
     """Launches go to the device of the tensors, whichever is current."""
     if device.type != "cuda":
         raise ValueError(f"the kernels take tensors on a GPU, not on {device}")
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+@functools.lru_cache(maxsize=1024)
+def _attention_workspace(batch: int, q_heads: int, kv_heads: int, dim: int, most: int, device: torch.device) -> int:
+    return _lib.load().tccl_decode_attention_workspace(batch, q_heads, kv_heads, dim, most)
 
 
 def _need(condition: bool, text: str) -> None:
@@ -45,7 +52,7 @@ def _need(condition: bool, text: str) -> None:
 
 
 def _integers(t: torch.Tensor, dtype: torch.dtype, shape, device: torch.device, name: str) -> None:
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or t.device != device or not t.is_contiguous():
+    if t.dtype != dtype or t.shape != shape or t.device != device or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {device}")
 
 
@@ -56,11 +63,13 @@ def _aligned(t: torch.Tensor, name: str) -> None:
 
 def _heads_first(t: torch.Tensor, name: str) -> Tuple[int, int]:
     """Strides (in elements) of a ``[tokens, heads, head_dim]`` tensor whose rows are whole and 16-byte aligned."""
+    if t.numel() == 0:
+        return 0, 0
+    token, head, element = t.stride()
     vec = 16 // t.element_size()
-    token, head = t.stride(0), t.stride(1)
-    if t.numel() and (t.stride(2) != 1 or token < 0 or head < 0 or token % vec or head % vec or t.data_ptr() % 16):
+    if element != 1 or token % vec or head % vec or t.data_ptr() % 16:
         raise ValueError(f"{name}: rows of head_dim elements must be contiguous and start at multiples of 16 bytes")
-    return (token, head) if t.numel() else (0, 0)
+    return token, head
 
 
 # ---------------------------------------------------------------- sum, per-head norm and rotation
@@ -68,21 +77,24 @@ def _heads_first(t: torch.Tensor, name: str) -> Tuple[int, int]:
 def _norm_arguments(tensor, q_weight, k_weight, positions, inv_freq, heads, what):
     dtype = _sum_dtype(tensor)
     dim = q_weight.numel()
-    _need(dim in HEAD_DIMS, f"{what}: head_dim (the weights' length) must be one of {HEAD_DIMS}")
-    _need(tensor.dim() == 2, f"{what}: the projection must be [tokens, columns]")
     device = tensor.device
-    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-        if w.dtype != tensor.dtype or w.shape != (dim,) or w.device != device or not w.is_contiguous():
-            raise ValueError(f"{what}: {name} must be a contiguous {tensor.dtype} tensor of shape ({dim},) on {device}")
-        _aligned(w, name)
+    if dim not in HEAD_DIMS:
+        raise ValueError(f"{what}: head_dim (the weights' length) must be one of {HEAD_DIMS}")
+    if tensor.dim() != 2:
+        raise ValueError(f"{what}: the projection must be [tokens, columns]")
+    for w in (q_weight, k_weight):
+        if w.dtype != tensor.dtype or w.shape != (dim,) or w.device != device or not w.is_contiguous() or w.data_ptr() % 16:
+            raise ValueError(f"{what}: the weights must be contiguous {tensor.dtype} tensors of shape ({dim},) on {device} that "
+                             "start at a multiple of 16 bytes")
     tokens, columns = tensor.shape
-    _need(all(n >= 0 for n in heads) and sum(heads) >= 1 and sum(heads) * dim == columns,
-          f"{what}: {columns} columns are not {heads[0]} + {heads[1]} + {heads[2]} heads of {dim}")
+    if min(heads) < 0 or sum(heads) < 1 or sum(heads) * dim != columns:
+        raise ValueError(f"{what}: {columns} columns are not {heads[0]} + {heads[1]} + {heads[2]} heads of {dim}")
     _integers(positions, torch.int64, (tokens,), device, "positions")
     if inv_freq.dim() != 1 or inv_freq.dtype != torch.float64 or inv_freq.device != device or not inv_freq.is_contiguous():
         raise ValueError(f"{what}: inv_freq must be a contiguous float64 vector on {device}")
     rotary = 2 * inv_freq.numel()
-    _need(rotary % 16 == 0 and rotary <= dim, f"{what}: 2 * len(inv_freq) must be a multiple of 16 and at most head_dim")
+    if rotary % 16 or rotary > dim:
+        raise ValueError(f"{what}: 2 * len(inv_freq) must be a multiple of 16 and at most head_dim")
     return dtype, dim, rotary
 
 
@@ -107,7 +119,7 @@ def qk_norm_rope(tensor: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.T
     lib = _lib.load()
     with spmd.collective():
         tokens = tensor.shape[0]
-        outs = [torch.empty((tokens, n, dim), dtype=tensor.dtype, device=tensor.device) for n in heads]
+        outs = [tensor.new_empty((tokens, n, dim)) for n in heads]
         if tokens == 0:                # (an empty view has no address to find a group by)
             return outs[0], outs[1], outs[2]
         symm = rendezvous(tensor)
@@ -230,7 +242,8 @@ def cache_read(cache: PagedCache, slots: torch.Tensor, *, dtype: torch.dtype = t
     _integers(slots, torch.int64, (tokens,), cache.device, "slots")
     _need(dtype in (torch.bfloat16, torch.float32), "cache_read returns bfloat16 or float32")
     if out is None:
-        k, v = (torch.empty(cache._rows(tokens), dtype=dtype, device=cache.device) for _ in range(2))
+        rows = cache._rows(tokens)
+        k, v = slots.new_empty(rows, dtype=dtype), slots.new_empty(rows, dtype=dtype)
     else:
         k, v = out
         for t, name in ((k, "out[0]"), (v, "out[1]")):
@@ -266,46 +279,44 @@ def decode_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tenso
     Returns ``[batch, q_heads, head_dim]`` bfloat16 and, with ``return_lse`` or ``lse``, the logarithm of the softmax's
     sum, float32 ``[batch, q_heads]``: what ``attention_all_reduce`` joins parts with.  A sequence without tokens gives
     0 and -inf.  Scores, softmax and sums are fp32; an infinite cached value gives NaN."""
-    batch = lengths.numel()
-    dim = cache.head_dim
-    _need(q.dtype == torch.bfloat16, "decode_attention takes bfloat16 queries")
-    if q.dim() != 3 or q.shape[0] != batch or q.shape[2] != dim or q.device != cache.device:
-        raise ValueError(f"q must be [{batch}, q_heads, {dim}] on {cache.device}")
+    batch, dim, device = lengths.numel(), cache.head_dim, cache.device
+    if q.dtype != torch.bfloat16 or q.dim() != 3 or q.shape[0] != batch or q.shape[2] != dim or q.device != device:
+        raise ValueError(f"q must be a bfloat16 tensor of shape [{batch}, q_heads, {dim}] on {device}")
     q_heads = q.shape[1]
-    _need(q_heads >= 1 and q_heads % cache.kv_heads == 0, "q_heads must be a multiple of the cache's kv_heads")
+    if q_heads < 1 or q_heads % cache.kv_heads:
+        raise ValueError("q_heads must be a multiple of the cache's kv_heads")
     q_strides = _heads_first(q, "q")
-    _integers(lengths, torch.int32, (batch,), cache.device, "lengths")
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != batch \
-            or page_table.device != cache.device:
-        raise ValueError(f"page_table must be an int32 tensor of shape [{batch}, pages] on {cache.device}")
-    width = page_table.shape[1]
-    _need(width <= 1 or page_table.stride(1) == 1, "page_table: a row must be contiguous")
-    _need(page_table.stride(0) >= 0, "page_table: rows must be in ascending order")
+    _integers(lengths, torch.int32, (batch,), device, "lengths")
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != batch or page_table.device != device:
+        raise ValueError(f"page_table must be an int32 tensor of shape [{batch}, pages] on {device}")
+    width, (row, element) = page_table.shape[1], page_table.stride()
+    if width > 1 and element != 1:
+        raise ValueError("page_table: a row must be contiguous")
     most = width * cache.page_size
     if max_length is not None:
-        _need(max_length >= 0, "max_length must not be negative")
+        if max_length < 0:
+            raise ValueError("max_length must not be negative")
         most = min(most, max_length)
-    _need(most < 1 << 31, "page_table has room for more than 2^31 tokens")
-    device = cache.device
+    if most >= 1 << 31:
+        raise ValueError("page_table has room for more than 2^31 tokens: give max_length")
     shape = (batch, q_heads, dim)
-    out = torch.empty(shape, dtype=torch.bfloat16, device=device) if out is None else _check_out(out, shape, q)
+    out = q.new_empty(shape) if out is None else _check_out(out, shape, q)
     if lse is not None:
         _integers(lse, torch.float32, (batch, q_heads), device, "lse")
     elif return_lse:
-        lse = torch.empty((batch, q_heads), dtype=torch.float32, device=device)
-    lib = _lib.load()
+        lse = q.new_empty((batch, q_heads), dtype=torch.float32)
     if scale is None:
         scale = 1.0 / math.sqrt(dim)
     with spmd.collective():
         if batch:
             _aligned(out, "out")
             with _on(device):
-                nbytes = lib.tccl_decode_attention_workspace(batch, q_heads, cache.kv_heads, dim, most)
-                workspace = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-                rc = lib.tccl_decode_attention(
-                    cache._ref, q.data_ptr(), *q_strides, page_table.data_ptr() or None, page_table.stride(0),
-                    lengths.data_ptr(), out.data_ptr(), lse.data_ptr() if lse is not None else None,
-                    workspace.data_ptr() if nbytes else None, nbytes, batch, q_heads, most, scale, _stream(device))
+                nbytes = _attention_workspace(batch, q_heads, cache.kv_heads, dim, most, device)
+                workspace = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+                rc = _lib.load().tccl_decode_attention(
+                    cache._ref, q.data_ptr(), *q_strides, page_table.data_ptr() or None, row, lengths.data_ptr(), out.data_ptr(),
+                    lse.data_ptr() if lse is not None else None, workspace.data_ptr() if nbytes else None, nbytes, batch, q_heads,
+                    most, scale, _stream(device))
             _lib.check("tccl_decode_attention", rc)
     return (out, lse) if lse is not None else out
 
@@ -320,7 +331,8 @@ def attention_all_reduce(tensor: torch.Tensor, lse: torch.Tensor, *, out: Option
     the joined output and its lse, the same on every rank.  A rank whose lse is -inf is left out, whatever its buffer
     holds; where all are, the output is 0 and lse -inf."""
     dtype = _sum_dtype(tensor)
-    _need(tensor.dim() >= 1 and tensor.shape[-1] in HEAD_DIMS, f"attention_all_reduce: head_dim must be one of {HEAD_DIMS}")
+    if tensor.dim() < 1 or tensor.shape[-1] not in HEAD_DIMS:
+        raise ValueError(f"attention_all_reduce: head_dim must be one of {HEAD_DIMS}")
     if lse.dtype != torch.float32 or lse.shape != tensor.shape[:-1] or lse.device != tensor.device:
         raise ValueError(f"lse must be a float32 tensor of shape {tuple(tensor.shape[:-1])} on {tensor.device}")
     lib = _lib.load()
@@ -330,8 +342,8 @@ def attention_all_reduce(tensor: torch.Tensor, lse: torch.Tensor, *, out: Option
         symm, symm_lse = rendezvous(tensor), rendezvous(lse)
         _refuse_remote(symm.group, "attention_all_reduce")
         _refuse_remote(symm_lse.group, "attention_all_reduce")
-        _need(symm.world_size == symm_lse.world_size and symm.rank == symm_lse.rank,
-              "attention_all_reduce: tensor and lse must be the same rank's buffers of two groups of one world")
+        if symm.world_size != symm_lse.world_size or symm.rank != symm_lse.rank:
+            raise ValueError("attention_all_reduce: tensor and lse must be the same rank's buffers of two groups of one world")
         symm.group.check_signals()
         output = torch.empty_like(tensor) if out is None else _check_out(out, tensor.shape, tensor)
         output_lse = torch.empty_like(lse)

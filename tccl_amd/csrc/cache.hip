@@ -3,16 +3,19 @@
 // page * page_size + place in the page; pages are numbered over all ranks, rank r holding pages
 // [r * pages_per_rank, (r + 1) * pages_per_rank).  The layout is described in rows.h.
 //
-// Both are moves: the floor is their bytes.  A workgroup takes 16 consecutive tokens of the list and one
-// head, eight elements per lane (2 * head_dim lanes).  Keys go between rows and 16-byte chunks directly;
-// values lie with their tokens innermost, so they pass through LDS, and what the workgroup's tokens do not
-// cover of a 16-byte group is left to element stores (write) or read along (read).
+// Both are moves: the floor is their bytes.  A workgroup takes TOKENS (64; 16 of a short list) consecutive
+// tokens of the list and one head.  Keys go between rows and 16-byte chunks directly.  Values lie with their tokens
+// innermost, in 16-byte groups of 8 or 16 tokens per dim: the list is cut into runs, tokens that follow each other
+// within one group, and a lane turns a run's 4 dims x 8 or 16 tokens in registers.  Reading takes a whole group and
+// uses the run's part of it; writing stores whole groups with one store per dim, and of others (a run that begins or
+// ends inside) what is whole of each four bytes, the rest element by element, since its neighbours may be
+// written by another workgroup.
 #include "host.h"
 #include "rows.h"
 
 namespace tccl {
 
-constexpr int kCacheTokens = 16;
+constexpr int kCacheBlock = 256;
 
 struct CacheArgs {
     PoolShape shape;
@@ -23,6 +26,80 @@ struct CacheArgs {
     size_t k_token, k_head, v_token, v_head;
     char *k_out, *v_out;
 };
+
+// Where the workgroup's tokens lie, and their runs.
+template <int TOKENS>
+struct Runs {
+    char *block[TOKENS]; // of the token's page and this head, nullptr: outside the pool
+    int place[TOKENS];   // in the page
+    int first[TOKENS], length[TOKENS];
+    int count;
+};
+
+// Run by the workgroup's first wave: lane i looks token i up.
+template <int GROUP, int TOKENS>
+__device__ __forceinline__ void find_runs(const CacheArgs &a, size_t begin, int h, Runs<TOKENS> &runs)
+{
+    const int lane = threadIdx.x;
+    const int64_t slot = lane < TOKENS && begin + lane < a.tokens ? a.slots[begin + lane] : -1;
+    char *const b = slot < 0 ? nullptr : a.shape.block(slot >> a.shape.page_shift, h);
+    const int64_t before = __shfl_up(slot, 1);
+    const bool live = b != nullptr;
+    const bool leads = live && (lane == 0 || before + 1 != slot || slot % GROUP == 0);
+    const uint64_t leaders = __ballot(leads), gaps = ~__ballot(live) | leaders;
+    if (lane < TOKENS) {
+        runs.block[lane] = b;
+        runs.place[lane] = static_cast<int>(slot & ((1 << a.shape.page_shift) - 1));
+    }
+    if (leads) {
+        const int n = __popcll(leaders & ((1ull << lane) - 1));
+        const uint64_t behind = lane == 63 ? 0 : gaps >> (lane + 1); // the next leader or token without a place
+        const int length = behind == 0 ? 64 - lane : __builtin_ctzll(behind) + 1;
+        runs.first[n] = lane;
+        runs.length[n] = length;
+    }
+    if (lane == 0) runs.count = __popcll(leaders);
+}
+
+// Four dwords as a 4 x 4 matrix of bytes, transposed.
+__device__ __forceinline__ void transpose_bytes(uint32_t &a, uint32_t &b, uint32_t &c, uint32_t &d)
+{
+    const uint32_t ab_low = __builtin_amdgcn_perm(b, a, 0x05010400u), ab_high = __builtin_amdgcn_perm(b, a, 0x07030602u);
+    const uint32_t cd_low = __builtin_amdgcn_perm(d, c, 0x05010400u), cd_high = __builtin_amdgcn_perm(d, c, 0x07030602u);
+    a = __builtin_amdgcn_perm(cd_low, ab_low, 0x05040100u);
+    b = __builtin_amdgcn_perm(cd_low, ab_low, 0x07060302u);
+    c = __builtin_amdgcn_perm(cd_high, ab_high, 0x05040100u);
+    d = __builtin_amdgcn_perm(cd_high, ab_high, 0x07060302u);
+}
+
+// A lane's part of a value group, 4 dims of GROUP tokens in 16 dwords: from by dim, as it is stored, to by token, or back
+// (`TO_TOKENS` false).
+template <class Store, bool TO_TOKENS>
+__device__ __forceinline__ void turn_group(const uint32_t (&in)[16], uint32_t (&out)[16])
+{
+    if constexpr (Store::kScaled) { // 16 tokens: dim i is dwords 4 i ..., token t is dword t
+#pragma unroll
+        for (int q = 0; q < 4; ++q) { // tokens 4 q ... 4 q + 3
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = TO_TOKENS ? in[4 * i + q] : in[4 * q + i];
+            transpose_bytes(w[0], w[1], w[2], w[3]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) out[TO_TOKENS ? 4 * q + i : 4 * i + q] = w[i];
+        }
+    } else { // 8 tokens: dim i is dwords 4 i ..., token t is dwords 2 t and 2 t + 1
+#pragma unroll
+        for (int q = 0; q < 4; ++q) // tokens 2 q and 2 q + 1
+#pragma unroll
+            for (int i = 0; i < 2; ++i) { // dims 2 i and 2 i + 1
+                const int dim0 = 4 * (2 * i) + q, dim1 = 4 * (2 * i + 1) + q;
+                const int token0 = 4 * q + i, token1 = 4 * q + 2 + i;
+                const uint32_t x = in[TO_TOKENS ? dim0 : token0], y = in[TO_TOKENS ? dim1 : token1];
+                out[TO_TOKENS ? token0 : dim0] = __builtin_amdgcn_perm(y, x, 0x05040100u);
+                out[TO_TOKENS ? token1 : dim1] = __builtin_amdgcn_perm(y, x, 0x07060302u);
+            }
+    }
+}
 
 // Largest finite magnitude of a lane's elements, as fp32 bits (order-preserving for magnitudes).
 __device__ __forceinline__ float finite_magnitude(const float *x)
@@ -38,213 +115,223 @@ __device__ __forceinline__ float finite_magnitude(const float *x)
 
 // Eight elements as they are stored: four dwords of bf16, or two of codes (and the row's scale byte).
 template <class Store, int LANES>
-__device__ __forceinline__ void encode(const float *x, uint32_t *code, uint32_t &scale)
+__device__ __forceinline__ void encode(const float *x, char *to, uint32_t &scale)
 {
     if constexpr (Store::kScaled) {
         scale = scale_byte(f32_to_bits(reduce_row<MaxOp, LANES>(finite_magnitude(x))));
         const float f = inverse_scale_of(scale);
+        u32x2 code;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            code[k] = pack_e4m3<false>(x[4 * k] * f, x[4 * k + 1] * f, 0);
-            code[k] = pack_e4m3<true>(x[4 * k + 2] * f, x[4 * k + 3] * f, code[k]);
+            const uint32_t half = pack_e4m3<false>(x[4 * k] * f, x[4 * k + 1] * f, 0);
+            code[k] = pack_e4m3<true>(x[4 * k + 2] * f, x[4 * k + 3] * f, half);
         }
+        if (to != nullptr) *reinterpret_cast<u32x2 *>(to) = code;
     } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) code[k] = pack_bf16(x[2 * k], x[2 * k + 1]);
+        if (to != nullptr) Bf16Row::store(to, x);
     }
 }
 
-template <class Row, class Store, int LANES>
-__global__ void __launch_bounds__(kCacheTokens * LANES)
+template <class Row, class Store, int LANES, int TOKENS>
+__global__ void __launch_bounds__(kCacheBlock)
 cache_write_kernel(CacheArgs a)
 {
-    constexpr int D = 8 * LANES, BYTES = Store::kBytes, GROUP = Store::kChunk, CODES = 2 * BYTES;
-    __shared__ __attribute__((aligned(16))) char values[kCacheTokens * D * BYTES];
-    __shared__ char *block[kCacheTokens];  // of the token's page and this head, nullptr: not written
-    __shared__ int place_in_page[kCacheTokens];
-    const int h = blockIdx.y, t = threadIdx.x / LANES, p = threadIdx.x % LANES;
-    const size_t first = static_cast<size_t>(blockIdx.x) * kCacheTokens;
+    constexpr int D = 8 * LANES, BYTES = Store::kBytes, GROUP = Store::kChunk, IN_DWORD = 4 / BYTES;
+    constexpr int ROUNDS = (TOKENS * LANES + kCacheBlock - 1) / kCacheBlock;
+    __shared__ __attribute__((aligned(16))) char values[TOKENS * D * BYTES];
+    __shared__ Runs<TOKENS> runs;
+    const int h = blockIdx.y, p = threadIdx.x % LANES;
+    const size_t begin = static_cast<size_t>(blockIdx.x) * TOKENS;
     const int page_size = 1 << a.shape.page_shift;
     const size_t v_at = static_cast<size_t>(page_size) * D * BYTES, scales_at = 2 * v_at;
-    if (threadIdx.x < kCacheTokens) {
-        const size_t i = first + threadIdx.x;
-        const int64_t slot = i < a.tokens ? a.slots[i] : -1;
-        block[threadIdx.x] = slot < 0 ? nullptr : a.shape.block(slot >> a.shape.page_shift, h);
-        place_in_page[threadIdx.x] = static_cast<int>(slot & (page_size - 1));
-    }
-    float k[8], v[8];
-    if (first + t < a.tokens) {
-        load_row<Row>(a.k + (first + t) * a.k_token + h * a.k_head + p * 8 * Row::kElemBytes, k);
-        load_row<Row>(a.v + (first + t) * a.v_token + h * a.v_head + p * 8 * Row::kElemBytes, v);
-    } else {
+    Row k[ROUNDS], v[ROUNDS];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) k[i] = v[i] = 0.0f;
+    for (int i = 0; i < ROUNDS; ++i) {
+        const int t = (threadIdx.x + i * kCacheBlock) / LANES;
+        if (t < TOKENS && begin + t < a.tokens) {
+            k[i].load(a.k + (begin + t) * a.k_token + h * a.k_head + p * 8 * Row::kElemBytes);
+            v[i].load(a.v + (begin + t) * a.v_token + h * a.v_head + p * 8 * Row::kElemBytes);
+        } else {
+            k[i].zero();
+            v[i].zero();
+        }
+    }
+    if (threadIdx.x < 64) find_runs<GROUP, TOKENS>(a, begin, h, runs);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < ROUNDS; ++i) {
+        const int t = (threadIdx.x + i * kCacheBlock) / LANES;
+        if (t >= TOKENS) break; // whole waves
+        char *const block = runs.block[t];
+        const int place = runs.place[t];
+        float x[8];
+        uint32_t k_scale = 0, v_scale = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = k[i].at(j);
+        encode<Store, LANES>(x,
+                             block == nullptr ? nullptr
+                                              : block + ((static_cast<size_t>(place >> 4) * (D / GROUP) + p * 8 / GROUP) * 16 +
+                                                         (place & 15)) * 16 + (p * 8 % GROUP) * BYTES,
+                             k_scale);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = v[i].at(j);
+        encode<Store, LANES>(x, values + (t * D + p * 8) * BYTES, v_scale);
+        if (Store::kScaled && block != nullptr && p == 0) {
+            block[scales_at + place] = static_cast<char>(k_scale);
+            block[scales_at + page_size + place] = static_cast<char>(v_scale);
+        }
     }
     __syncthreads();
-    char *const mine = block[t];
-    const int place = place_in_page[t];
-    uint32_t code[CODES], k_scale = 0, v_scale = 0;
-    encode<Store, LANES>(k, code, k_scale);
-    if (mine != nullptr) {
-        char *dst = mine + ((static_cast<size_t>(place >> 4) * (D / GROUP) + p * 8 / GROUP) * 16 + (place & 15)) * 16 +
-                    (p * 8 % GROUP) * BYTES;
-        if constexpr (Store::kScaled)
-            *reinterpret_cast<u32x2 *>(dst) = u32x2{code[0], code[1]};
-        else
-            *reinterpret_cast<u32x4 *>(dst) = u32x4{code[0], code[1], code[2], code[3]};
-    }
-    encode<Store, LANES>(v, code, v_scale);
-    {
-        char *dst = values + (t * D + p * 8) * BYTES;
-        if constexpr (Store::kScaled)
-            *reinterpret_cast<u32x2 *>(dst) = u32x2{code[0], code[1]};
-        else
-            *reinterpret_cast<u32x4 *>(dst) = u32x4{code[0], code[1], code[2], code[3]};
-    }
-    if (Store::kScaled && mine != nullptr && p == 0) {
-        mine[scales_at + place] = static_cast<char>(k_scale);
-        mine[scales_at + page_size + place] = static_cast<char>(v_scale);
-    }
-    __syncthreads();
-    // values: lane = dim, one group of GROUP tokens of the list at a time
-    for (int item = threadIdx.x; item < D * (kCacheTokens / GROUP); item += kCacheTokens * LANES) {
-        const int dim = item % D, t0 = item / D * GROUP;
-        char *const b = block[t0];
-        const int at = place_in_page[t0];
-        bool whole = b != nullptr && at % GROUP == 0;
+    for (int item = threadIdx.x; item < runs.count * (D / 4); item += kCacheBlock) {
+        const int n = item / (D / 4), dim = item % (D / 4) * 4;
+        const int first = runs.first[n], length = runs.length[n], place = runs.place[first], start = place % GROUP;
+        uint32_t by_token[16], by_dim[16];
 #pragma unroll
-        for (int i = 1; i < GROUP; ++i) whole = whole && block[t0 + i] == b && place_in_page[t0 + i] == at + i;
-        if (whole) {
-            u32x4 out;
-            if constexpr (Store::kScaled) {
+        for (int t = 0; t < GROUP; ++t) {
+            // tokens of the group that are not in the run: any of its own, which are not stored there
+            const int at = first + (t < start ? 0 : (t < start + length ? t - start : length - 1));
+            const char *src = values + (at * D + dim) * BYTES;
+#pragma unroll
+            for (int w = 0; w < BYTES; ++w) by_token[t * BYTES + w] = reinterpret_cast<const uint32_t *>(src)[w];
+        }
+        turn_group<Store, false>(by_token, by_dim);
+        char *const to = runs.block[first] + v_at + (static_cast<size_t>(place / GROUP) * D + dim) * 16;
+        if (length == GROUP) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                store_vec<false>(to, i, u32x4{by_dim[4 * i], by_dim[4 * i + 1], by_dim[4 * i + 2], by_dim[4 * i + 3]});
+            continue;
+        }
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const int low = w * IN_DWORD; // the dword's first token
+            if (low >= start && low + IN_DWORD <= start + length) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) *reinterpret_cast<uint32_t *>(to + i * 16 + w * 4) = by_dim[4 * i + w];
+                continue;
+            }
+#pragma unroll
+            for (int t = 0; t < IN_DWORD; ++t) {
+                if (low + t < start || low + t >= start + length) continue;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    uint32_t u = 0;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        u |= static_cast<uint32_t>(static_cast<uint8_t>(values[(t0 + 4 * i + j) * D + dim])) << (8 * j);
-                    out[i] = u;
+                    const uint32_t x = by_dim[4 * i + w] >> (8 * BYTES * t);
+                    if constexpr (Store::kScaled)
+                        to[i * 16 + low + t] = static_cast<char>(x);
+                    else
+                        *reinterpret_cast<uint16_t *>(to + i * 16 + (low + t) * 2) = static_cast<uint16_t>(x);
                 }
-            } else {
-                const uint16_t *src = reinterpret_cast<const uint16_t *>(values) + t0 * D + dim;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    out[i] = static_cast<uint32_t>(src[2 * i * D]) | static_cast<uint32_t>(src[(2 * i + 1) * D]) << 16;
-            }
-            store_vec<false>(b + v_at, static_cast<size_t>(at / GROUP) * D + dim, out);
-        } else {
-            for (int i = 0; i < GROUP; ++i) {
-                char *const bi = block[t0 + i];
-                if (bi == nullptr) continue;
-                const int pi = place_in_page[t0 + i];
-                const size_t to = (static_cast<size_t>(pi / GROUP) * D + dim) * 16 + pi % GROUP * BYTES;
-                if constexpr (Store::kScaled)
-                    bi[v_at + to] = values[(t0 + i) * D + dim];
-                else
-                    *reinterpret_cast<uint16_t *>(bi + v_at + to) =
-                        reinterpret_cast<const uint16_t *>(values)[(t0 + i) * D + dim];
             }
         }
     }
 }
 
-// Eight stored elements (codes of a row with one scale) in fp32.
-template <class Store>
+// N (4 or 8) stored elements of a row with one scale, in fp32.
+template <class Store, int N>
 __device__ __forceinline__ void decode(const uint32_t *code, float scale, float *x)
 {
     if constexpr (Store::kScaled) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            x[4 * k] = __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(code[k]), 0) * scale;
-            x[4 * k + 1] = __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(code[k]), 1) * scale;
-            x[4 * k + 2] = __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(code[k]), 2) * scale;
-            x[4 * k + 3] = __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(code[k]), 3) * scale;
+        for (int k = 0; k < N / 4; ++k) {
+            const f32x2 low = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(code[k]), false);
+            const f32x2 high = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(code[k]), true);
+            x[4 * k] = low.x * scale;
+            x[4 * k + 1] = low.y * scale;
+            x[4 * k + 2] = high.x * scale;
+            x[4 * k + 3] = high.y * scale;
         }
     } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < N / 2; ++k) {
             x[2 * k] = bits_to_f32(code[k] << 16);
             x[2 * k + 1] = bits_to_f32(code[k] & 0xFFFF0000u);
         }
     }
 }
 
-template <class Row, class Store, int LANES>
-__global__ void __launch_bounds__(kCacheTokens * LANES)
+// Four elements of a row.
+template <class Row>
+__device__ __forceinline__ void store_four(char *to, const float *x)
+{
+    if constexpr (Row::kElemBytes == 2)
+        *reinterpret_cast<u32x2 *>(to) = u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
+    else
+        store_vec<false>(to, 0, u32x4{f32_to_bits(x[0]), f32_to_bits(x[1]), f32_to_bits(x[2]), f32_to_bits(x[3])});
+}
+
+template <class Row, class Store, int LANES, int TOKENS>
+__global__ void __launch_bounds__(kCacheBlock)
 cache_read_kernel(CacheArgs a)
 {
-    constexpr int D = 8 * LANES, BYTES = Store::kBytes, GROUP = Store::kChunk, CODES = 2 * BYTES;
-    // one 16-byte value group per dim for each different group that the tokens lie in; a dim more per 16 keeps
-    // the transposed reads off one bank
-    __shared__ u32x4 groups[kCacheTokens][D];
-    __shared__ const char *block[kCacheTokens];
-    __shared__ int place_in_page[kCacheTokens], group_of[kCacheTokens], leader[kCacheTokens];
-    __shared__ int count;
-    const int h = blockIdx.y, t = threadIdx.x / LANES, p = threadIdx.x % LANES;
-    const size_t first = static_cast<size_t>(blockIdx.x) * kCacheTokens;
+    constexpr int D = 8 * LANES, BYTES = Store::kBytes, GROUP = Store::kChunk, CHUNKS = D / GROUP;
+    constexpr int ROUNDS = (TOKENS * CHUNKS + kCacheBlock - 1) / kCacheBlock;
+    __shared__ Runs<TOKENS> runs;
+    const int h = blockIdx.y;
+    const size_t begin = static_cast<size_t>(blockIdx.x) * TOKENS;
     const int page_size = 1 << a.shape.page_shift;
     const size_t v_at = static_cast<size_t>(page_size) * D * BYTES, scales_at = 2 * v_at;
-    if (threadIdx.x < 64) { // one whole wave: tokens are its first 16 lanes
-        const size_t i = first + threadIdx.x;
-        const int64_t slot = threadIdx.x < kCacheTokens && i < a.tokens ? a.slots[i] : -1;
-        const char *b = slot < 0 ? nullptr : a.shape.block(slot >> a.shape.page_shift, h);
-        const int place = static_cast<int>(slot & (page_size - 1));
-        // a token leads a group unless the token before it lies in the same one
-        const int64_t key = b == nullptr ? -1 : slot / GROUP;
-        const int64_t before = __shfl_up(key, 1);
-        const bool leads = key >= 0 && (threadIdx.x == 0 || before != key);
-        const uint64_t mask = __ballot(leads);
-        if (threadIdx.x < kCacheTokens) {
-            block[threadIdx.x] = b;
-            place_in_page[threadIdx.x] = place;
-            const int n = __popcll(mask & ((2ull << threadIdx.x) - 1)) - 1;
-            group_of[threadIdx.x] = n;
-            if (leads) leader[n] = threadIdx.x;
-        }
-        if (threadIdx.x == 0) count = __popcll(mask);
-    }
+    const size_t token_bytes = static_cast<size_t>(a.shape.heads) * D * Row::kElemBytes;
+    const size_t to = begin * token_bytes + static_cast<size_t>(h) * D * Row::kElemBytes;
+    if (threadIdx.x < 64) find_runs<GROUP, TOKENS>(a, begin, h, runs);
     __syncthreads();
-    for (int item = threadIdx.x; item < count * D; item += kCacheTokens * LANES) {
-        const int n = item / D, dim = item % D, l = leader[n];
-        groups[n][dim] = load_vec<false>(block[l] + v_at, static_cast<size_t>(place_in_page[l] / GROUP) * D + dim);
-    }
-    const char *const mine = block[t];
-    const int place = place_in_page[t];
-    uint32_t code[CODES] = {};
-    float k_scale = 0.0f, v_scale = 0.0f, x[8];
-    if (mine != nullptr) {
-        const char *src = mine +
-                          ((static_cast<size_t>(place >> 4) * (D / GROUP) + p * 8 / GROUP) * 16 + (place & 15)) * 16 +
-                          (p * 8 % GROUP) * BYTES;
+    const int here = a.tokens - begin < TOKENS ? static_cast<int>(a.tokens - begin) : TOKENS;
+    u32x4 k[ROUNDS];
+    uint32_t k_scale[ROUNDS];
 #pragma unroll
-        for (int i = 0; i < CODES; ++i) code[i] = reinterpret_cast<const uint32_t *>(src)[i];
-        if constexpr (Store::kScaled) {
-            k_scale = scale_of(static_cast<uint8_t>(mine[scales_at + place]));
-            v_scale = scale_of(static_cast<uint8_t>(mine[scales_at + page_size + place]));
+    for (int i = 0; i < ROUNDS; ++i) {
+        const int t = (threadIdx.x + i * kCacheBlock) / CHUNKS, c = (threadIdx.x + i * kCacheBlock) % CHUNKS;
+        k[i] = u32x4{0, 0, 0, 0};
+        k_scale[i] = 0;
+        if (t >= here) continue;
+        const char *const block = runs.block[t];
+        const int place = runs.place[t];
+        if (block == nullptr) continue;
+        k[i] = load_vec<false>(block, (static_cast<size_t>(place >> 4) * CHUNKS + c) * 16 + (place & 15));
+        if constexpr (Store::kScaled) k_scale[i] = static_cast<uint8_t>(block[scales_at + place]);
+    }
+    for (int item = threadIdx.x; item < runs.count * (D / 4); item += kCacheBlock) {
+        const int n = item / (D / 4), dim = item % (D / 4) * 4;
+        const int first = runs.first[n], length = runs.length[n], place = runs.place[first], start = place % GROUP;
+        const char *const from = runs.block[first] + v_at + (static_cast<size_t>(place / GROUP) * D + dim) * 16;
+        uint32_t by_dim[16], by_token[16];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const u32x4 u = load_vec<false>(from, i);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) by_dim[4 * i + w] = u[w];
+        }
+        u32x4 scales = {};
+        if constexpr (Store::kScaled)
+            scales = load_vec<false>(runs.block[first] + scales_at + page_size + (place - start), 0);
+        turn_group<Store, true>(by_dim, by_token);
+        char *const out = a.v_out + to + dim * Row::kElemBytes;
+#pragma unroll
+        for (int t = 0; t < GROUP; ++t) {
+            if (t < start || t >= start + length) continue;
+            float x[4];
+            decode<Store, 4>(by_token + t * BYTES, scale_of((scales[(t >> 2) & 3] >> (8 * (t & 3))) & 0xFFu), x);
+            store_four<Row>(out + (first + t - start) * token_bytes, x);
         }
     }
-    const bool live = first + t < a.tokens;
-    const size_t to = (((first + t) * a.shape.heads + h) * D + p * 8) * Row::kElemBytes;
-    decode<Store>(code, k_scale, x);
-    if (live) Row::store(a.k_out + to, x);
-    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < CODES; ++i) code[i] = 0;
-    if (mine != nullptr) {
-        const int within = place % GROUP;
-        const u32x4 *row = groups[group_of[t]];
+    for (int i = 0; i < ROUNDS; ++i) {
+        const int t = (threadIdx.x + i * kCacheBlock) / CHUNKS, c = (threadIdx.x + i * kCacheBlock) % CHUNKS;
+        if (t >= here) continue;
+        const uint32_t code[4] = {k[i][0], k[i][1], k[i][2], k[i][3]};
+        char *const out = a.k_out + to + t * token_bytes + c * GROUP * Row::kElemBytes;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if constexpr (Store::kScaled)
-                code[i >> 2] |= static_cast<uint32_t>(reinterpret_cast<const uint8_t *>(row + p * 8 + i)[within])
-                                << (8 * (i & 3));
-            else
-                code[i >> 1] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t *>(row + p * 8 + i)[within])
-                                << (16 * (i & 1));
+        for (int part = 0; part < GROUP / 8; ++part) {
+            float x[8];
+            decode<Store, 8>(code + 2 * part, scale_of(k_scale[i]), x);
+            Row::store(out + part * 8 * Row::kElemBytes, x);
+        }
+        if (runs.block[t] == nullptr) { // no run: the token's values are zeros as well
+            char *const v_out = a.v_out + to + t * token_bytes + c * GROUP * Row::kElemBytes;
+            const float zeros[8] = {};
+#pragma unroll
+            for (int part = 0; part < GROUP / 8; ++part) Row::store(v_out + part * 8 * Row::kElemBytes, zeros);
         }
     }
-    decode<Store>(code, v_scale, x);
-    if (live) Row::store(a.v_out + to, x);
 }
 
 static size_t block_bytes_of(const tccl_paged_cache &c)
@@ -280,15 +367,24 @@ int check_cache(const tccl_paged_cache *c, PoolShape *shape)
     return TCCL_OK;
 }
 
+template <class Row, class Store, int LANES, int TOKENS>
+static hipError_t launch_cache_tokens(bool write, const CacheArgs &a, hipStream_t stream)
+{
+    const dim3 grid(static_cast<unsigned>((a.tokens + TOKENS - 1) / TOKENS), a.shape.heads);
+    if (write)
+        hipLaunchKernelGGL((cache_write_kernel<Row, Store, LANES, TOKENS>), grid, dim3(kCacheBlock), 0, stream, a);
+    else
+        hipLaunchKernelGGL((cache_read_kernel<Row, Store, LANES, TOKENS>), grid, dim3(kCacheBlock), 0, stream, a);
+    return hipGetLastError();
+}
+
+// Tiles of 64 tokens where they fill the GPU twice, else of 16.
 template <class Row, class Store, int LANES>
 static hipError_t launch_cache(bool write, const CacheArgs &a, hipStream_t stream)
 {
-    const dim3 grid(static_cast<unsigned>((a.tokens + kCacheTokens - 1) / kCacheTokens), a.shape.heads);
-    if (write)
-        hipLaunchKernelGGL((cache_write_kernel<Row, Store, LANES>), grid, dim3(kCacheTokens * LANES), 0, stream, a);
-    else
-        hipLaunchKernelGGL((cache_read_kernel<Row, Store, LANES>), grid, dim3(kCacheTokens * LANES), 0, stream, a);
-    return hipGetLastError();
+    if (a.tokens / 64 * a.shape.heads >= static_cast<size_t>(compute_units()) * 2)
+        return launch_cache_tokens<Row, Store, LANES, 64>(write, a, stream);
+    return launch_cache_tokens<Row, Store, LANES, 16>(write, a, stream);
 }
 
 template <class Row, class Store>
