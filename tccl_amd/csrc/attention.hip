@@ -497,49 +497,56 @@ struct JoinArgs {
     char *to;
     float *to_lse;
     size_t rows;
-    int lane_shift; // log2 of the lanes of a row
+    int vec_shift; // log2 of the 16-byte vectors of a row
 };
 
-// out = sum_i w_i o_i / sum_i w_i, w_i = exp(lse_i - max lse): W reads and one write per element, so a
-// grid-stride pass with every source's load in flight; a row whose lse is -inf is not used, whatever it holds.
-template <class Row, int NSRC>
+// out = sum_i w_i o_i / sum_i w_i, w_i = exp(lse_i - max lse): W reads and one write per element, a vector per lane
+// with every source's load in flight, read once and so marked as streaming; a row whose lse is -inf is not used,
+// whatever it holds.
+template <class Sum, int NSRC>
 __global__ void __launch_bounds__(256)
 attention_join_kernel(JoinArgs<NSRC> a)
 {
-    const size_t items = a.rows << a.lane_shift;
+    constexpr int N = kVecBytes / Sum::kElemBytes;
+    const size_t items = a.rows << a.vec_shift;
     for (size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x; i < items;
          i += static_cast<size_t>(gridDim.x) * 256) {
-        const size_t row = i >> a.lane_shift;
-        Row in[NSRC];
+        const size_t row = i >> a.vec_shift;
+        u32x4 in[NSRC];
         float w[NSRC];
 #pragma unroll
-        for (int s = 0; s < NSRC; ++s) w[s] = a.lse[s][row];
+        for (int s = 0; s < NSRC; ++s) in[s] = load_vec<true>(a.out[s], i);
 #pragma unroll
-        for (int s = 0; s < NSRC; ++s) in[s].load(a.out[s] + i * 8 * Row::kElemBytes);
+        for (int s = 0; s < NSRC; ++s) w[s] = a.lse[s][row];
         float best = w[0];
 #pragma unroll
         for (int s = 1; s < NSRC; ++s) best = fmaxf(best, w[s]);
-        float total = 0.0f, o[8] = {};
+        float total = 0.0f, o[N] = {};
 #pragma unroll
         for (int s = 0; s < NSRC; ++s) {
             if (w[s] == -__builtin_inff()) continue;
             const float f = expf(w[s] - best);
             total = total + f;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) o[k] = __builtin_fmaf(in[s].at(k), f, o[k]);
+            for (int k = 0; k < N; ++k) {
+                const uint32_t u = N == 4 ? in[s][k & 3] : ((k & 1) ? in[s][k >> 1] & 0xFFFF0000u : in[s][k >> 1] << 16);
+                o[k] = __builtin_fmaf(bits_to_f32(u), f, o[k]);
+            }
         }
         const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+        u32x4 r;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) o[k] = o[k] * inv;
-        Row::store(a.to + i * 8 * Row::kElemBytes, o);
-        if ((i & ((static_cast<size_t>(1) << a.lane_shift) - 1)) == 0)
+        for (int k = 0; k < 4; ++k)
+            r[k] = N == 4 ? f32_to_bits(o[k] * inv) : pack_bf16(o[2 * k % N] * inv, o[(2 * k + 1) % N] * inv);
+        store_vec<false>(a.to, i, r);
+        if ((i & ((static_cast<size_t>(1) << a.vec_shift) - 1)) == 0)
             a.to_lse[row] = total == 0.0f ? -__builtin_inff() : best + logf(total);
     }
 }
 
-template <class Row, int NSRC>
+template <class Sum, int NSRC>
 static hipError_t launch_join(const void *const *outs, const void *const *lses, void *to, float *to_lse, size_t rows,
-                              int lane_shift, hipStream_t stream)
+                              int dim, hipStream_t stream)
 {
     JoinArgs<NSRC> a = {};
     for (int i = 0; i < NSRC; ++i) {
@@ -549,26 +556,26 @@ static hipError_t launch_join(const void *const *outs, const void *const *lses, 
     a.to = static_cast<char *>(to);
     a.to_lse = to_lse;
     a.rows = rows;
-    a.lane_shift = lane_shift;
-    const size_t need = ((rows << lane_shift) + 255) / 256, most = static_cast<size_t>(compute_units()) * 8;
-    hipLaunchKernelGGL((attention_join_kernel<Row, NSRC>), dim3(static_cast<unsigned>(need < most ? need : most)),
+    a.vec_shift = __builtin_ctz(dim * Sum::kElemBytes / kVecBytes);
+    const size_t need = ((rows << a.vec_shift) + 255) / 256, most = static_cast<size_t>(compute_units()) * 8;
+    hipLaunchKernelGGL((attention_join_kernel<Sum, NSRC>), dim3(static_cast<unsigned>(need < most ? need : most)),
                        dim3(256), 0, stream, a);
     return hipGetLastError();
 }
 
-template <class Row>
+template <class Sum>
 static hipError_t launch_join_nsrc(const void *const *outs, const void *const *lses, int world, void *to,
-                                   float *to_lse, size_t rows, int lane_shift, hipStream_t s)
+                                   float *to_lse, size_t rows, int dim, hipStream_t s)
 {
     switch (world) {
-    case 1: return launch_join<Row, 1>(outs, lses, to, to_lse, rows, lane_shift, s);
-    case 2: return launch_join<Row, 2>(outs, lses, to, to_lse, rows, lane_shift, s);
-    case 3: return launch_join<Row, 3>(outs, lses, to, to_lse, rows, lane_shift, s);
-    case 4: return launch_join<Row, 4>(outs, lses, to, to_lse, rows, lane_shift, s);
-    case 5: return launch_join<Row, 5>(outs, lses, to, to_lse, rows, lane_shift, s);
-    case 6: return launch_join<Row, 6>(outs, lses, to, to_lse, rows, lane_shift, s);
-    case 7: return launch_join<Row, 7>(outs, lses, to, to_lse, rows, lane_shift, s);
-    case 8: return launch_join<Row, 8>(outs, lses, to, to_lse, rows, lane_shift, s);
+    case 1: return launch_join<Sum, 1>(outs, lses, to, to_lse, rows, dim, s);
+    case 2: return launch_join<Sum, 2>(outs, lses, to, to_lse, rows, dim, s);
+    case 3: return launch_join<Sum, 3>(outs, lses, to, to_lse, rows, dim, s);
+    case 4: return launch_join<Sum, 4>(outs, lses, to, to_lse, rows, dim, s);
+    case 5: return launch_join<Sum, 5>(outs, lses, to, to_lse, rows, dim, s);
+    case 6: return launch_join<Sum, 6>(outs, lses, to, to_lse, rows, dim, s);
+    case 7: return launch_join<Sum, 7>(outs, lses, to, to_lse, rows, dim, s);
+    case 8: return launch_join<Sum, 8>(outs, lses, to, to_lse, rows, dim, s);
     default: return hipErrorInvalidValue;
     }
 }
@@ -710,9 +717,8 @@ extern "C" int tccl_attention_all_reduce(const void *const *outs, const void *co
         if (!aligned16(outs[i]) || !aligned16(lses[i])) return TCCL_EALIGN;
     }
     if (rows == 0) return TCCL_OK;
-    const int shift = head_dim == 64 ? 3 : (head_dim == 128 ? 4 : 5);
     hipStream_t s = static_cast<hipStream_t>(stream);
     return hip_code(dtype == TCCL_BF16
-                        ? launch_join_nsrc<Bf16Row>(outs, lses, world, out, lse, rows, shift, s)
-                        : launch_join_nsrc<F32Row>(outs, lses, world, out, lse, rows, shift, s));
+                        ? launch_join_nsrc<Bf16Sum>(outs, lses, world, out, lse, rows, head_dim, s)
+                        : launch_join_nsrc<F32Sum>(outs, lses, world, out, lse, rows, head_dim, s));
 }

@@ -139,7 +139,7 @@ qk_norm_rope_kernel(NormArgs<NSRC> a)
 #pragma unroll
         for (int i = 0; i < NSRC; ++i) {
             if (live)
-                in[i].load(a.src[i] + at);
+                in[i].template load<true>(a.src[i] + at);
             else
                 in[i].zero();
         }
@@ -200,12 +200,12 @@ qk_norm_rope_backward_kernel(NormArgs<NSRC> a)
 #pragma unroll
             for (int i = 0; i < NSRC; ++i) {
                 if (live && !is_v)
-                    in[i].load(a.src[i] + at);
+                    in[i].template load<true>(a.src[i] + at);
                 else
                     in[i].zero();
             }
             if (live)
-                dg.load(dy + ((token * mine + (head - before)) * D + place * 8) * Row::kElemBytes);
+                dg.template load<true>(dy + ((token * mine + (head - before)) * D + place * 8) * Row::kElemBytes);
             else
                 dg.zero();
             float x[8], g[8];
@@ -254,24 +254,28 @@ qk_norm_rope_backward_kernel(NormArgs<NSRC> a)
     }
 }
 
-// The partial rows in order: 16 columns per workgroup, 16 row lanes each, joined through LDS.
-__global__ void __launch_bounds__(256)
+// The partial rows in a fixed order: 16 columns per workgroup, every 64th row per lane with its loads in
+// flight, joined through LDS.
+constexpr int kGradRows = 64;
+__global__ void __launch_bounds__(16 * kGradRows)
 weight_grad_kernel(const float *partial, int rows, int dim, float *dq_weight, float *dk_weight)
 {
-    __shared__ float part[16][17];
+    __shared__ float part[kGradRows][17];
     const int column = blockIdx.x * 16 + (threadIdx.x & 15), lane = threadIdx.x >> 4;
     float s = 0.0f;
-    for (int r = lane; r < rows; r += 16) s = s + partial[static_cast<size_t>(r) * 2 * dim + column];
+#pragma unroll 16
+    for (int r = lane; r < rows; r += kGradRows) s = s + partial[static_cast<size_t>(r) * 2 * dim + column];
     part[lane][threadIdx.x & 15] = s;
     __syncthreads();
-    if (lane == 0) {
-        float sum = 0.0f;
-        for (int r = 0; r < 16; ++r) sum = sum + part[r][threadIdx.x];
-        if (column < dim)
-            dq_weight[column] = sum;
-        else
-            dk_weight[column - dim] = sum;
-    }
+    if (lane >= 4) return;
+    for (int r = lane + 4; r < kGradRows; r += 4) s = s + part[r][threadIdx.x & 15];
+    s = s + __shfl_xor(s, 16);
+    s = s + __shfl_xor(s, 32);
+    if (lane > 0) return;
+    if (column < dim)
+        dq_weight[column] = s;
+    else
+        dk_weight[column - dim] = s;
 }
 
 struct NormCall {
@@ -455,7 +459,7 @@ extern "C" int tccl_qk_norm_rope_backward(const void *const *bufs, int world, co
         if (e != hipSuccess) return hip_code(e);
     }
     // no tokens: no partial rows, and the weight gradients are zero
-    hipLaunchKernelGGL(weight_grad_kernel, dim3(2 * head_dim / 16), dim3(256), 0, s, c.partial,
+    hipLaunchKernelGGL(weight_grad_kernel, dim3(2 * head_dim / 16), dim3(16 * kGradRows), 0, s, c.partial,
                        static_cast<int>(c.workgroups), head_dim, dq_weight, dk_weight);
     return hip_code(hipGetLastError());
 }
