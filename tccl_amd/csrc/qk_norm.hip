@@ -114,6 +114,10 @@ __device__ __forceinline__ void fill_angles(const NormArgs<NSRC> &a, f32x2 *turn
     }
 }
 
+// A wave reads up to three items (a token's heads, 512 elements at a time) before it works on the first: 8 sources of
+// 50 MB 81 us with one at a time, 80 two, 78 three, 81 four; one fp32 source of 168 MB 66, 66, 62, 62.
+constexpr int kNormItems = 3;
+
 template <class Row, int LANES, int NSRC>
 __global__ void __launch_bounds__(kNormBlock)
 qk_norm_rope_kernel(NormArgs<NSRC> a)
@@ -129,38 +133,52 @@ qk_norm_rope_kernel(NormArgs<NSRC> a)
     load_row<Row>(a.weight[1] + place * 8 * Row::kElemBytes, wk);
     fill_angles(a, turn, first);
     __syncthreads();
-    for (int item = wave; item < groups * a.tokens_per_wg; item += kNormWaves) {
-        const int local = item / groups;
-        const size_t token = first + local;
-        const int head = (item - local * groups) * HEADS + lane / LANES;
-        const bool live = token < a.tokens && head < all;
-        const size_t at = ((token * all + head) * D + place * 8) * Row::kElemBytes;
-        Row in[NSRC];
+    for (int item0 = wave; item0 < groups * a.tokens_per_wg; item0 += kNormWaves * kNormItems) {
+        float xs[kNormItems][8];
 #pragma unroll
-        for (int i = 0; i < NSRC; ++i) {
-            if (live)
-                in[i].template load<true>(a.src[i] + at);
-            else
-                in[i].zero();
+        for (int u = 0; u < kNormItems; ++u) {
+            const int item = item0 + u * kNormWaves;
+            const int local = item / groups;
+            const size_t token = first + local;
+            const int head = (item - local * groups) * HEADS + lane / LANES;
+            const bool live = item < groups * a.tokens_per_wg && token < a.tokens && head < all;
+            const size_t at = ((token * all + head) * D + place * 8) * Row::kElemBytes;
+            Row in[NSRC];
+#pragma unroll
+            for (int i = 0; i < NSRC; ++i) {
+                if (live)
+                    in[i].template load<true>(a.src[i] + at);
+                else
+                    in[i].zero();
+            }
+            sum_sources<Row, NSRC>(in, xs[u]);
         }
-        float x[8];
-        sum_sources<Row, NSRC>(in, x);
-        const float r = inverse_rms<LANES>(x, a.eps);
-        const bool is_q = head < a.heads[0], is_v = head >= a.heads[0] + a.heads[1];
-        float y[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) y[k] = x[k] * r * (is_q ? wq[k] : wk[k]);
-        rotate<LANES, 1>(y, turn + local * (a.rotary >> 1), place, a.rotary, a.interleaved != 0);
-        if (is_v) {
+        for (int u = 0; u < kNormItems; ++u) {
+            const int item = item0 + u * kNormWaves;
+            if (item >= groups * a.tokens_per_wg) break;
+            const int local = item / groups;
+            const size_t token = first + local;
+            const int head = (item - local * groups) * HEADS + lane / LANES;
+            const bool live = token < a.tokens && head < all;
+            const float *x = xs[u];
+            const float r = inverse_rms<LANES>(x, a.eps);
+            const bool is_q = head < a.heads[0], is_v = head >= a.heads[0] + a.heads[1];
+            float y[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) y[k] = x[k];
-        }
-        if (live) {
-            const int kind = is_q ? 0 : (is_v ? 2 : 1);
-            const int before = is_q ? 0 : (is_v ? a.heads[0] + a.heads[1] : a.heads[0]);
-            char *out = is_q ? a.out[0] : (is_v ? a.out[2] : a.out[1]);
-            const int mine = is_q ? a.heads[0] : (kind == 2 ? a.heads[2] : a.heads[1]);
-            Row::store(out + ((token * mine + (head - before)) * D + place * 8) * Row::kElemBytes, y);
+            for (int k = 0; k < 8; ++k) y[k] = x[k] * r * (is_q ? wq[k] : wk[k]);
+            rotate<LANES, 1>(y, turn + local * (a.rotary >> 1), place, a.rotary, a.interleaved != 0);
+            if (is_v) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) y[k] = x[k];
+            }
+            if (live) {
+                const int kind = is_q ? 0 : (is_v ? 2 : 1);
+                const int before = is_q ? 0 : (is_v ? a.heads[0] + a.heads[1] : a.heads[0]);
+                char *out = is_q ? a.out[0] : (is_v ? a.out[2] : a.out[1]);
+                const int mine = is_q ? a.heads[0] : (kind == 2 ? a.heads[2] : a.heads[1]);
+                Row::store(out + ((token * mine + (head - before)) * D + place * 8) * Row::kElemBytes, y);
+            }
         }
     }
 }
