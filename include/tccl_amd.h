@@ -495,7 +495,7 @@ int tccl_cache_read(const tccl_paged_cache *cache, const int64_t *slots, size_t 
 /* Attention of one new token per sequence: q [batch][q_heads][head_dim] bf16 (strides in elements, whole 16-byte
  * vectors), q_heads a multiple of the cache's kv_heads (query head i reads key head i / (q_heads / kv_heads)).
  * Token t of sequence b lies on page page_table[b * page_table_stride + t / page_size]; a sequence has
- * min(lengths[b], max_tokens) tokens, and page_table rows must reach that far.  Tokens on a page
+ * min(lengths[b], max_tokens) tokens (max_tokens at most 2^30), and page_table rows must reach that far.  Tokens on a page
  * outside the pool are left out.  out [batch][q_heads][head_dim] bf16 and lse [batch][q_heads] (natural log, may
  * be NULL); without tokens out is 0 and lse -inf.  `workspace`: tccl_decode_attention_workspace() bytes for the same
  * sizes (may be 0), written before they are read; not to be shared by calls that may run at the same time. */

@@ -297,8 +297,8 @@ def decode_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tenso
         if max_length < 0:
             raise ValueError("max_length must not be negative")
         most = min(most, max_length)
-    if most >= 1 << 31:
-        raise ValueError("page_table has room for more than 2^31 tokens: give max_length")
+    if most > 1 << 30:
+        raise ValueError("page_table has room for more than 2^30 tokens: give max_length")
     shape = (batch, q_heads, dim)
     out = q.new_empty(shape) if out is None else _check_out(out, shape, q)
     if lse is not None:

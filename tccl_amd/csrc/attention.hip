@@ -647,7 +647,8 @@ static hipError_t launch_attention_dim(const AttnArgs &a, int dim, hipStream_t s
 
 static int check_attention_shape(size_t batch, int q_heads, int kv_heads, int most)
 {
-    if (q_heads < 1 || q_heads > 65536 || kv_heads < 1 || q_heads % kv_heads != 0 || most < 0) return TCCL_EINVAL;
+    if (q_heads < 1 || q_heads > 65536 || kv_heads < 1 || q_heads % kv_heads != 0) return TCCL_EINVAL;
+    if (most < 0 || most > (1 << 30)) return TCCL_EINVAL;
     if (batch > (static_cast<size_t>(1) << 20)) return TCCL_EINVAL;
     return TCCL_OK;
 }
@@ -680,7 +681,7 @@ extern "C" int tccl_decode_attention(const tccl_paged_cache *cache, const void *
     if (batch == 0) return TCCL_OK;
     const AttnPlan plan = plan_attention(batch, q_heads, cache->kv_heads, cache->head_dim, max_tokens);
     if (plan.workspace > 0 && (workspace == nullptr || workspace_bytes < plan.workspace)) return TCCL_ESCRATCH;
-    if (batch * plan.head_groups > 0x7FFFFFFFull || batch * q_heads > 0x7FFFFFFFull) return TCCL_EINVAL;
+    if (!fits_launch(plan.workgroups > 0 ? batch * q_heads : batch * plan.head_groups, kAttnBlock)) return TCCL_EINVAL;
     a.q = static_cast<const char *>(q);
     a.table = page_table;
     a.table_row = page_table_stride;

@@ -408,7 +408,7 @@ static hipError_t launch_cache_types(bool write, const CacheArgs &a, const tccl_
                                 : launch_cache_dim<F32Row, Bf16Store>(write, a, c.head_dim, stream);
 }
 
-constexpr size_t kMostTokens = static_cast<size_t>(1) << 31;
+constexpr size_t kMostTokens = static_cast<size_t>(1) << 29; // as many tiles of 64 are one launch
 
 } // namespace tccl
 

@@ -26,6 +26,9 @@ inline int dtype_size(int dtype)
 // Number of compute units of the current device (cached per process; 256 on MI355X).
 int compute_units();
 
+// Whether `grid` workgroups of `block` threads are one launch: a dimension has at most 2^32 - 1 threads.
+inline bool fits_launch(size_t grid, size_t block) { return grid <= 0xFFFFFFFFull / block; }
+
 // A resolved launch shape.
 struct Shape {
     int block, unroll, grid, tile_iters;

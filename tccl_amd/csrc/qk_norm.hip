@@ -397,7 +397,8 @@ static int check_norm(const NormCall &c, int dtype)
     if (!(c.eps >= 0.0f)) return TCCL_EINVAL;
     if (c.weight[0] == nullptr || c.weight[1] == nullptr || c.positions == nullptr) return TCCL_EINVAL;
     if (c.rotary > 0 && c.inv_freq == nullptr) return TCCL_EINVAL;
-    if (c.tokens > (static_cast<size_t>(1) << 31) - 1) return TCCL_EINVAL; // one workgroup per token at most
+    if (!c.backward && !fits_launch(c.tokens, kNormBlock)) return TCCL_EINVAL; // one workgroup per token at most
+    if (c.tokens > 0x7FFFFFFFull) return TCCL_EINVAL;
     if (!aligned16(c.weight[0]) || !aligned16(c.weight[1])) return TCCL_EALIGN;
     for (int i = 0; i < c.world; ++i) {
         if (c.bufs[i] == nullptr) return TCCL_EINVAL;

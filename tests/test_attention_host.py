@@ -50,6 +50,7 @@ def test_norm_entry_points_check_their_arguments():
            dict(v=None), dict(qw=None), dict(kw=None), dict(pos=None), dict(inv=None), dict(dim=96), dict(rotary=8),
            dict(rotary=80), dict(rotary=-16), dict(heads=(0, 0, 0)), dict(heads=(-1, 2, 2)), dict(eps=-1.0),
            dict(eps=math.nan), dict(dtype=2), dict(dtype=7), dict(tokens=1 << 31)]
+    assert fwd(tokens=1 << 24) == EINVAL                      # more workgroups than one launch has
     for kw in bad:
         assert fwd(**kw) == EINVAL, kw
         assert bwd(**kw) == EINVAL, kw
@@ -85,7 +86,7 @@ def test_cache_entry_points_check_their_arguments():
     assert write(desc(bufs=None)) == EINVAL and read(desc(bufs=None)) == EINVAL
     assert write(desc(bufs=0x20008)) == EALIGN and read(desc(bufs=0x20008)) == EALIGN
     assert write(desc()) == OK and read(desc()) == OK
-    for kw in (dict(k=None), dict(v=None), dict(slots=None), dict(dtype=2), dict(tokens=(1 << 31) + 1)):
+    for kw in (dict(k=None), dict(v=None), dict(slots=None), dict(dtype=2), dict(tokens=(1 << 29) + 1)):
         assert write(desc(), **kw) == EINVAL and read(desc(), **kw) == EINVAL, kw
     assert write(desc(), k=0x1008) == EALIGN and read(desc(), v=0x2004) == EALIGN
     assert write(desc(), strides=(256, 60, 256, 64)) == EALIGN and write(desc(), strides=(256, 64, 257, 64)) == EALIGN
@@ -101,12 +102,13 @@ def test_attention_entry_points_check_their_arguments():
     assert attn(desc()) == OK
     assert attn(desc(), lse=None) == OK                       # no lse wanted
     assert attn(desc(), table=None, most=0) == OK             # no sequence can have a token
-    for kw in (dict(q=None), dict(lengths=None), dict(out=None), dict(table=None), dict(heads=6), dict(heads=0), dict(most=-1),
+    for kw in (dict(q=None), dict(lengths=None), dict(out=None), dict(table=None), dict(heads=6), dict(heads=0), dict(most=-1), dict(most=(1 << 30) + 1),
                dict(batch=(1 << 20) + 1)):
         assert attn(desc(), **kw) == EINVAL, kw
     assert attn(desc(page_size=20)) == EINVAL and attn(None) == EINVAL
     for kw in (dict(q=0x1008), dict(out=0x4008), dict(ws=0x6004), dict(strides=(512, 60)), dict(strides=(508, 64))):
         assert attn(desc(), **kw) == EALIGN, kw
+    assert attn(desc(kv_heads=64), batch=1 << 20, heads=64, most=64) == EINVAL   # more workgroups than one launch has
     need = lib.tccl_decode_attention_workspace(1, 8, 4, 64, 100_000)
     assert need > 0
     assert attn(desc(), batch=1, most=100_000) == ESCRATCH
