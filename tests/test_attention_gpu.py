@@ -244,6 +244,12 @@ CACHE_CASES = [
     (4, 1, 256, 1, 128, BF16, F32),
     (5, 5, 16, 2, 256, BF16, BF16),
     (1, 9, 16, 8, 64, E4M3, F32),
+    # enough tokens for the larger tiles
+    (8, 40, 64, 8, 64, E4M3, BF16),
+    (4, 70, 128, 4, 128, BF16, BF16),
+    (2, 50, 256, 2, 256, E4M3, F32),
+    (1, 700, 16, 6, 64, BF16, F32),
+    (3, 200, 32, 2, 128, E4M3, F32),
 ]
 
 
@@ -427,6 +433,8 @@ ATTENTION_CASES = [
     (1, [530, 0] + [3] * 300, 2, 2, 64, 16, E4M3),
     (3, [5, 0, 17, 1] * 1100, 1, 1, 64, 16, BF16),
     (1, [600] + [0, 3] * 2100, 2, 1, 64, 16, BF16),
+    (2, [20011] + [0, 1] * 2050, 2, 1, 64, 16, E4M3),
+    (2, [600, 3, 0] * 700, 1, 1, 64, 16, BF16),
 ]
 
 
