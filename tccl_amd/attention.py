@@ -32,18 +32,29 @@ _STORES = {torch.bfloat16: _lib.TCCL_BF16, torch.float8_e4m3fn: _lib.TCCL_E4M3}
 
 
 _HERE = contextlib.nullcontext()
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _collective():
+    """``spmd.collective()`` where the caller is a rank of a per-rank program, else nothing to wait for."""
+    return _HERE if spmd.current_rank() is None else spmd.collective()
 
 
 def _on(device: torch.device):
     """Launches go to the device of the tensors, whichever is current."""
     if device.type != "cuda":
         raise ValueError(f"the kernels take tensors on a GPU, not on {device}")
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == _current_device() else torch.cuda.device(device)
 
 
 @functools.lru_cache(maxsize=1024)
 def _attention_workspace(batch: int, q_heads: int, kv_heads: int, dim: int, most: int, device: torch.device) -> int:
     return _lib.load().tccl_decode_attention_workspace(batch, q_heads, kv_heads, dim, most)
+
+
+@functools.lru_cache(maxsize=64)
+def _grad_workspace(dim: int, device: torch.device) -> int:
+    return _lib.load().tccl_qk_norm_rope_backward_workspace(dim)
 
 
 def _need(condition: bool, text: str) -> None:
@@ -117,7 +128,7 @@ def qk_norm_rope(tensor: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.T
     heads = (q_heads, k_heads, v_heads)
     dtype, dim, rotary = _norm_arguments(tensor, q_weight, k_weight, positions, inv_freq, heads, "qk_norm_rope")
     lib = _lib.load()
-    with spmd.collective():
+    with _collective():
         tokens = tensor.shape[0]
         outs = [tensor.new_empty((tokens, n, dim)) for n in heads]
         if tokens == 0:                # (an empty view has no address to find a group by)
@@ -147,13 +158,13 @@ def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor, dv: torch.Tensor, 
     heads = tuple(g.shape[1] if g.dim() == 3 else -1 for g in (dq, dk, dv))
     dtype, dim, rotary = _norm_arguments(tensor, q_weight, k_weight, positions, inv_freq, heads, "qk_norm_rope_backward")
     tokens = tensor.shape[0]
-    for g, n, name in zip((dq, dk, dv), heads, ("dq", "dk", "dv")):
-        if g.shape != (tokens, n, dim) or g.dtype != tensor.dtype or g.device != tensor.device or not g.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous {tensor.dtype} tensor of shape {(tokens, n, dim)} on {tensor.device}")
-        if g.numel():
-            _aligned(g, name)
+    for g, n in zip((dq, dk, dv), heads):
+        if g.shape != (tokens, n, dim) or g.dtype != tensor.dtype or g.device != tensor.device or not g.is_contiguous() \
+                or (g.data_ptr() % 16 and g.numel()):
+            raise ValueError(f"dq, dk and dv must be contiguous {tensor.dtype} tensors of shape [{tokens}, heads, {dim}] on "
+                             f"{tensor.device} that start at a multiple of 16 bytes")
     lib = _lib.load()
-    with spmd.collective():
+    with _collective():
         device = tensor.device
         dx = torch.empty_like(tensor)
         if tokens == 0:
@@ -161,17 +172,17 @@ def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor, dv: torch.Tensor, 
         symm = rendezvous(tensor)
         _refuse_remote(symm.group, "qk_norm_rope_backward")
         symm.group.check_signals()
-        dweights = torch.empty((2, dim), dtype=torch.float32, device=device)
+        dweights = tensor.new_empty((2, dim), dtype=torch.float32)
         with _on(device):
-            nbytes = lib.tccl_qk_norm_rope_backward_workspace(dim)
-            workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            nbytes = _grad_workspace(dim, device)
+            workspace = tensor.new_empty(nbytes, dtype=torch.uint8)
             first = dweights.data_ptr()
             rc = lib.tccl_qk_norm_rope_backward(
                 symm.buffer_ptrs_host, symm.world_size, *(g.data_ptr() or None for g in (dq, dk, dv)), q_weight.data_ptr(),
                 k_weight.data_ptr(), positions.data_ptr(), inv_freq.data_ptr() or None, dx.data_ptr(), first, first + 4 * dim,
                 workspace.data_ptr(), nbytes, tokens, *heads, dim, rotary, int(interleaved), eps, dtype, _stream(device))
         _lib.check("tccl_qk_norm_rope_backward", rc)
-    return dx, dweights[0], dweights[1]
+    return (dx, *dweights.unbind(0))
 
 
 # ---------------------------------------------------------------- the paged cache
@@ -250,7 +261,7 @@ def cache_read(cache: PagedCache, slots: torch.Tensor, *, dtype: torch.dtype = t
             if t.shape != cache._rows(tokens) or t.dtype != dtype or t.device != cache.device or not t.is_contiguous():
                 raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {cache._rows(tokens)} on {cache.device}")
     code = _sum_dtype(k)
-    with spmd.collective():
+    with _collective():
         if tokens:
             _aligned(k, "out[0]")
             _aligned(v, "out[1]")
@@ -300,14 +311,17 @@ def decode_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tenso
     if most > 1 << 30:
         raise ValueError("page_table has room for more than 2^30 tokens: give max_length")
     shape = (batch, q_heads, dim)
-    out = q.new_empty(shape) if out is None else _check_out(out, shape, q)
+    if out is None:
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
+    else:
+        _check_out(out, shape, q)
     if lse is not None:
         _integers(lse, torch.float32, (batch, q_heads), device, "lse")
     elif return_lse:
         lse = q.new_empty((batch, q_heads), dtype=torch.float32)
     if scale is None:
         scale = 1.0 / math.sqrt(dim)
-    with spmd.collective():
+    with _collective():
         if batch:
             _aligned(out, "out")
             with _on(device):
@@ -336,7 +350,7 @@ def attention_all_reduce(tensor: torch.Tensor, lse: torch.Tensor, *, out: Option
     if lse.dtype != torch.float32 or lse.shape != tensor.shape[:-1] or lse.device != tensor.device:
         raise ValueError(f"lse must be a float32 tensor of shape {tuple(tensor.shape[:-1])} on {tensor.device}")
     lib = _lib.load()
-    with spmd.collective():
+    with _collective():
         if lse.numel() == 0:           # (an empty view has no address to find a group by)
             return torch.empty_like(tensor) if out is None else _check_out(out, tensor.shape, tensor), torch.empty_like(lse)
         symm, symm_lse = rendezvous(tensor), rendezvous(lse)
