@@ -11,6 +11,8 @@
 // elements, so a wave works on 512 consecutive elements (four heads of 128) with one 16-byte load per
 // source; the mean is a reduction over head_dim / 8 lanes in registers.  Angles are formed in fp64 turns
 // (fp32 would lose the fraction of a far position's angle) once per token by the workgroup, into LDS.
+#include <type_traits>
+
 #include "host.h"
 #include "rows.h"
 
@@ -46,6 +48,16 @@ __device__ __forceinline__ f32x2 rotation(int64_t position, double inv_freq)
     return f32x2{cospif(half_turns), sinpif(half_turns)};
 }
 
+// The workgroup's (cos, sin) pairs, [token][rotary / 2], and kTurns behind them (cos, -sin).  A lane needs `each` = 8
+// pairs that follow each other (4 where neighbours are pairs); two of them are one 16-byte read, and these lie
+// lane by lane, so that a row's reads, and those of the lanes that take the other sign, fall into different banks.
+constexpr int kTurns = kNormTokens * kMaxRotary / 2 + 16;
+__device__ __forceinline__ int turn_place(int pair, int each, int lanes)
+{
+    const int lane = pair / each, k = pair % each;
+    return ((k >> 1) * lanes + lane) * 2 + (k & 1);
+}
+
 // A lane's eight elements, rotated (SIGN = 1) or rotated back (-1); `place` is the lane's place in its row.
 template <int LANES, int SIGN>
 __device__ __forceinline__ void rotate(float *x, const f32x2 *turn, int place, int rotary, bool interleaved)
@@ -53,30 +65,34 @@ __device__ __forceinline__ void rotate(float *x, const f32x2 *turn, int place, i
     const int lanes = rotary >> 3;
     if (interleaved) {
         if (place < lanes) {
+            const f32x2 *t = turn + (SIGN < 0 ? kTurns : 0) + 2 * place;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const f32x2 cs = turn[4 * place + k];
-                const float s = SIGN * cs.y, a = x[2 * k], b = x[2 * k + 1];
-                x[2 * k] = __builtin_fmaf(a, cs.x, -(b * s));
-                x[2 * k + 1] = __builtin_fmaf(b, cs.x, a * s);
+                const f32x2 cs = t[(k >> 1) * 2 * lanes + (k & 1)];
+                const float u = x[2 * k], v = x[2 * k + 1];
+                x[2 * k] = __builtin_fmaf(u, cs.x, -(v * cs.y));
+                x[2 * k + 1] = __builtin_fmaf(v, cs.x, u * cs.y);
             }
         }
     } else {
         const int half = lanes >> 1;
         const bool low = place < half;
-        const int other = place >= lanes ? place : (low ? place + half : place - half);
-        const int lane = threadIdx.x & 63;
-        const int from = (lane & ~(LANES - 1)) + other;
-        float y[8];
+        float y[8]; // the other half's
+        if (LANES == 16 && lanes == LANES) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) y[k] = __shfl(x[k], from);
+            for (int k = 0; k < 8; ++k) y[k] = dpp<kDppRotate8>(x[k]);
+        } else {
+            const int lane = threadIdx.x & 63;
+            const int from = (lane & ~(LANES - 1)) + (place >= lanes ? place : (low ? place + half : place - half));
+#pragma unroll
+            for (int k = 0; k < 8; ++k) y[k] = __shfl(x[k], from);
+        }
         if (place < lanes) {
-            const f32x2 *t = turn + 8 * (low ? place : place - half);
+            const f32x2 *t = turn + (low == (SIGN > 0) ? kTurns : 0) + 2 * (low ? place : place - half);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                const f32x2 cs = t[k];
-                const float s = SIGN * (low ? -cs.y : cs.y);
-                x[k] = __builtin_fmaf(x[k], cs.x, y[k] * s);
+                const f32x2 cs = t[(k >> 1) * 2 * half + (k & 1)];
+                x[k] = __builtin_fmaf(x[k], cs.x, y[k] * cs.y);
             }
         }
     }
@@ -103,15 +119,29 @@ __device__ __forceinline__ float inverse_rms(const float *x, float eps)
     return rsqrtf(__builtin_fmaf(reduce_row<AddOp, LANES>(s), 1.0f / (8 * LANES), eps));
 }
 
-// The angles of the workgroup's tokens, [token][rotary / 2].
+// The angles of the workgroup's tokens.  A place behind the last token is no rotation (and not what LDS happens to
+// hold: a missing token's zeros have to stay zeros).
 template <int NSRC>
 __device__ __forceinline__ void fill_angles(const NormArgs<NSRC> &a, f32x2 *turn, size_t first)
 {
     const int half = a.rotary >> 1;
     for (int i = threadIdx.x; i < half * a.tokens_per_wg; i += kNormBlock) {
         const size_t t = first + i / half;
-        if (t < a.tokens) turn[i] = rotation(a.positions[t], a.inv_freq[i % half]);
+        const f32x2 cs = t < a.tokens ? rotation(a.positions[t], a.inv_freq[i % half]) : f32x2{1.0f, 0.0f};
+        const int each = a.interleaved ? 4 : 8, to = i / half * half + turn_place(i % half, each, half / each);
+        turn[to] = cs;
+        turn[kTurns + to] = f32x2{cs.x, -cs.y};
     }
+}
+
+// What the heads of an item are: of one kind, which the whole wave then works on without asking, or mixed.
+enum Kind { kQuery, kKey, kValue, kMixed };
+template <int NSRC>
+__device__ __forceinline__ Kind kind_of(const NormArgs<NSRC> &a, int head0, int heads)
+{
+    const int q = a.heads[0], qk = a.heads[0] + a.heads[1], all = qk + a.heads[2];
+    const int last = (head0 + heads < all ? head0 + heads : all) - 1;
+    return last < q ? kQuery : (head0 >= qk ? kValue : (head0 >= q && last < qk ? kKey : kMixed));
 }
 
 // A wave reads up to three items (a token's heads, 512 elements at a time) before it works on the first: 8 sources of
@@ -122,32 +152,31 @@ template <class Row, int LANES, int NSRC>
 __global__ void __launch_bounds__(kNormBlock)
 qk_norm_rope_kernel(NormArgs<NSRC> a)
 {
-    constexpr int D = 8 * LANES, HEADS = 64 / LANES; // heads a wave holds
-    __shared__ f32x2 turn[kNormTokens * kMaxRotary / 2];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, place = lane & (LANES - 1);
+    constexpr int D = 8 * LANES, HEADS = 64 / LANES, BYTES = Row::kElemBytes; // heads a wave holds
+    __shared__ __attribute__((aligned(16))) f32x2 turn[2 * kTurns];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), place = lane & (LANES - 1);
+    const uint32_t mine_at = lane * 8 * BYTES; // heads follow each other: the lane's elements of an item
     const int all = a.heads[0] + a.heads[1] + a.heads[2];
-    const int groups = (all + HEADS - 1) / HEADS;
+    const int groups = (all + HEADS - 1) / HEADS, items = groups * a.tokens_per_wg;
     const size_t first = static_cast<size_t>(blockIdx.x) * a.tokens_per_wg;
     float wq[8], wk[8];
-    load_row<Row>(a.weight[0] + place * 8 * Row::kElemBytes, wq);
-    load_row<Row>(a.weight[1] + place * 8 * Row::kElemBytes, wk);
+    load_row<Row>(a.weight[0] + place * 8 * BYTES, wq);
+    load_row<Row>(a.weight[1] + place * 8 * BYTES, wk);
     fill_angles(a, turn, first);
     __syncthreads();
-    for (int item0 = wave; item0 < groups * a.tokens_per_wg; item0 += kNormWaves * kNormItems) {
+    for (int item0 = wave; item0 < items; item0 += kNormWaves * kNormItems) {
         float xs[kNormItems][8];
 #pragma unroll
         for (int u = 0; u < kNormItems; ++u) {
             const int item = item0 + u * kNormWaves;
-            const int local = item / groups;
-            const size_t token = first + local;
-            const int head = (item - local * groups) * HEADS + lane / LANES;
-            const bool live = item < groups * a.tokens_per_wg && token < a.tokens && head < all;
-            const size_t at = ((token * all + head) * D + place * 8) * Row::kElemBytes;
+            const int local = item / groups, head0 = (item - local * groups) * HEADS;
+            const size_t token = first + local, at = (token * all + head0) * D * BYTES;
+            const bool live = item < items && token < a.tokens && head0 + lane / LANES < all;
             Row in[NSRC];
 #pragma unroll
             for (int i = 0; i < NSRC; ++i) {
                 if (live)
-                    in[i].template load<true>(a.src[i] + at);
+                    in[i].template load<true>(a.src[i] + at + mine_at);
                 else
                     in[i].zero();
             }
@@ -156,28 +185,34 @@ qk_norm_rope_kernel(NormArgs<NSRC> a)
 #pragma unroll
         for (int u = 0; u < kNormItems; ++u) {
             const int item = item0 + u * kNormWaves;
-            if (item >= groups * a.tokens_per_wg) break;
-            const int local = item / groups;
+            if (item >= items) break;
+            const int local = item / groups, head0 = (item - local * groups) * HEADS, head = head0 + lane / LANES;
             const size_t token = first + local;
-            const int head = (item - local * groups) * HEADS + lane / LANES;
             const bool live = token < a.tokens && head < all;
-            const float *x = xs[u];
-            const float r = inverse_rms<LANES>(x, a.eps);
-            const bool is_q = head < a.heads[0], is_v = head >= a.heads[0] + a.heads[1];
-            float y[8];
+            float *x = xs[u];
+            auto work = [&](auto kind) {
+                constexpr Kind KIND = decltype(kind)::value;
+                const bool is_q = KIND == kQuery || (KIND == kMixed && head < a.heads[0]);
+                const bool is_v = KIND == kValue || (KIND == kMixed && head >= a.heads[0] + a.heads[1]);
+                if constexpr (KIND != kValue) {
+                    const float r = inverse_rms<LANES>(x, a.eps);
+                    float y[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) y[k] = x[k] * r * (is_q ? wq[k] : wk[k]);
-            rotate<LANES, 1>(y, turn + local * (a.rotary >> 1), place, a.rotary, a.interleaved != 0);
-            if (is_v) {
+                    for (int k = 0; k < 8; ++k) y[k] = x[k] * r * (is_q ? wq[k] : wk[k]);
+                    rotate<LANES, 1>(y, turn + local * (a.rotary >> 1), place, a.rotary, a.interleaved != 0);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) y[k] = x[k];
-            }
-            if (live) {
-                const int kind = is_q ? 0 : (is_v ? 2 : 1);
+                    for (int k = 0; k < 8; ++k) x[k] = is_v ? x[k] : y[k];
+                }
                 const int before = is_q ? 0 : (is_v ? a.heads[0] + a.heads[1] : a.heads[0]);
-                char *out = is_q ? a.out[0] : (is_v ? a.out[2] : a.out[1]);
-                const int mine = is_q ? a.heads[0] : (kind == 2 ? a.heads[2] : a.heads[1]);
-                Row::store(out + ((token * mine + (head - before)) * D + place * 8) * Row::kElemBytes, y);
+                const int mine = is_q ? a.heads[0] : (is_v ? a.heads[2] : a.heads[1]);
+                char *const out = is_q ? a.out[0] : (is_v ? a.out[2] : a.out[1]);
+                if (live) Row::store(out + (token * mine + (head0 - before)) * D * BYTES + mine_at, x);
+            };
+            switch (kind_of(a, head0, HEADS)) {
+            case kQuery: work(std::integral_constant<Kind, kQuery>()); break;
+            case kKey: work(std::integral_constant<Kind, kKey>()); break;
+            case kValue: work(std::integral_constant<Kind, kValue>()); break;
+            default: work(std::integral_constant<Kind, kMixed>()); break;
             }
         }
     }
@@ -186,69 +221,97 @@ qk_norm_rope_kernel(NormArgs<NSRC> a)
 // Workgroups walk the tokens with the grid's stride; each lane keeps the weight gradients of its eight dims
 // in registers until the end, so that a workgroup leaves one partial row and the result does not depend on
 // the order in which workgroups finish.
+// Workgroups that run at once on a compute unit: as many as the registers allow (8,192 tokens of 48 heads of 128, one
+// bf16 source: 51 us with five, 57 with four; six spill).
+constexpr int kMostGradPerUnit = 5;
+template <class Row, int NSRC>
+constexpr int kGradPerUnit = (Row::kElemBytes == 2 ? 5 : 4) - (NSRC > 6 ? 1 : 0);
+
 template <class Row, int LANES, int NSRC>
-__global__ void __launch_bounds__(kNormBlock)
+__global__ void __launch_bounds__(kNormBlock, (kGradPerUnit<Row, NSRC>))
 qk_norm_rope_backward_kernel(NormArgs<NSRC> a)
 {
-    constexpr int D = 8 * LANES, HEADS = 64 / LANES;
-    __shared__ f32x2 turn[kNormTokens * kMaxRotary / 2];
+    constexpr int D = 8 * LANES, HEADS = 64 / LANES, BYTES = Row::kElemBytes;
+    __shared__ __attribute__((aligned(16))) f32x2 turn[2 * kTurns];
     __shared__ float sums[kNormWaves][2][D];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, place = lane & (LANES - 1);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), place = lane & (LANES - 1);
+    const uint32_t mine_at = lane * 8 * BYTES; // heads follow each other: the lane's elements of an item
     const int all = a.heads[0] + a.heads[1] + a.heads[2];
-    const int groups = (all + HEADS - 1) / HEADS;
-    float wq[8], wk[8];
-    load_row<Row>(a.weight[0] + place * 8 * Row::kElemBytes, wq);
-    load_row<Row>(a.weight[1] + place * 8 * Row::kElemBytes, wk);
+    const int groups = (all + HEADS - 1) / HEADS, items = groups * a.tokens_per_wg;
+    Row wq, wk;
+    wq.load(a.weight[0] + place * 8 * BYTES);
+    wk.load(a.weight[1] + place * 8 * BYTES);
     float dw[2][8] = {};
     for (size_t first = static_cast<size_t>(blockIdx.x) * a.tokens_per_wg; first < a.tokens;
          first += static_cast<size_t>(gridDim.x) * a.tokens_per_wg) {
         fill_angles(a, turn, first);
         __syncthreads();
-        for (int item = wave; item < groups * a.tokens_per_wg; item += kNormWaves) {
-            const int local = item / groups;
-            const size_t token = first + local;
-            const int head = (item - local * groups) * HEADS + lane / LANES;
+        for (int item = wave; item < items; item += kNormWaves) {
+            const int local = item / groups, head0 = (item - local * groups) * HEADS, head = head0 + lane / LANES;
+            const size_t token = first + local, at = (token * all + head0) * D * BYTES;
             const bool live = token < a.tokens && head < all;
-            const bool is_q = head < a.heads[0], is_v = head >= a.heads[0] + a.heads[1];
-            const int before = is_q ? 0 : (is_v ? a.heads[0] + a.heads[1] : a.heads[0]);
-            const int mine = is_q ? a.heads[0] : (is_v ? a.heads[2] : a.heads[1]);
-            const char *dy = is_q ? a.grad[0] : (is_v ? a.grad[2] : a.grad[1]);
-            const size_t at = ((token * all + head) * D + place * 8) * Row::kElemBytes;
-            Row in[NSRC], dg;
+            auto work = [&](auto kind) {
+                constexpr Kind KIND = decltype(kind)::value;
+                const bool is_q = KIND == kQuery || (KIND == kMixed && head < a.heads[0]);
+                const bool is_v = KIND == kValue || (KIND == kMixed && head >= a.heads[0] + a.heads[1]);
+                const int before = is_q ? 0 : (is_v ? a.heads[0] + a.heads[1] : a.heads[0]);
+                const int mine = is_q ? a.heads[0] : (is_v ? a.heads[2] : a.heads[1]);
+                const char *const from = is_q ? a.grad[0] : (is_v ? a.grad[2] : a.grad[1]);
+                Row in[NSRC], dy;
 #pragma unroll
-            for (int i = 0; i < NSRC; ++i) {
-                if (live && !is_v)
-                    in[i].template load<true>(a.src[i] + at);
+                for (int i = 0; i < NSRC; ++i) {
+                    if (KIND != kValue && live && !is_v)
+                        in[i].template load<true>(a.src[i] + at + mine_at);
+                    else
+                        in[i].zero();
+                }
+                if (live)
+                    dy.template load<true>(from + (token * mine + (head0 - before)) * D * BYTES + mine_at);
                 else
-                    in[i].zero();
-            }
-            if (live)
-                dg.template load<true>(dy + ((token * mine + (head - before)) * D + place * 8) * Row::kElemBytes);
-            else
-                dg.zero();
-            float x[8], g[8];
-            sum_sources<Row, NSRC>(in, x);
+                    dy.zero();
+                float g[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) g[k] = dg.at(k);
-            const float r = inverse_rms<LANES>(x, a.eps);
-            rotate<LANES, -1>(g, turn + local * (a.rotary >> 1), place, a.rotary, a.interleaved != 0);
-            float dot = 0.0f;
+                for (int k = 0; k < 8; ++k) g[k] = dy.at(k);
+                auto weight = [&](int k) {
+                    if constexpr (KIND == kQuery) return wq.at(k);
+                    if constexpr (KIND == kKey) return wk.at(k);
+                    const float q = wq.at(k), k_ = wk.at(k);
+                    return is_q ? q : k_;
+                };
+                if constexpr (KIND != kValue) {
+                    float n[8], dot = 0.0f;
+                    sum_sources<Row, NSRC>(in, n);
+                    const float r = inverse_rms<LANES>(n, a.eps);
+                    rotate<LANES, -1>(g, turn + local * (a.rotary >> 1), place, a.rotary, a.interleaved != 0);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float n = x[k] * r, gn = g[k] * n;
-                dot = __builtin_fmaf(gn, is_q ? wq[k] : wk[k], dot);
-                // a value head's (and a missing head's) x is zero here, and so is its gn
-                dw[0][k] = dw[0][k] + (is_q ? gn : 0.0f);
-                dw[1][k] = dw[1][k] + (is_q || is_v ? 0.0f : gn);
-            }
-            dot = reduce_row<AddOp, LANES>(dot) * (1.0f / D);
-            float d[8];
+                    for (int k = 0; k < 8; ++k) {
+                        n[k] = n[k] * r;
+                        const float gn = g[k] * n[k];
+                        g[k] = g[k] * weight(k);
+                        dot = __builtin_fmaf(g[k], n[k], dot);
+                        // a value head's (and a missing head's) x is zero here, and so is its gn
+                        if constexpr (KIND == kMixed) {
+                            dw[0][k] = dw[0][k] + (is_q ? gn : 0.0f);
+                            dw[1][k] = dw[1][k] + (is_q || is_v ? 0.0f : gn);
+                        } else {
+                            dw[KIND == kQuery ? 0 : 1][k] = dw[KIND == kQuery ? 0 : 1][k] + gn;
+                        }
+                    }
+                    dot = reduce_row<AddOp, LANES>(dot) * (1.0f / D);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float n = x[k] * r, u = g[k] * (is_q ? wq[k] : wk[k]);
-                d[k] = is_v ? dg.at(k) : r * __builtin_fmaf(-n, dot, u);
+                    for (int k = 0; k < 8; ++k) {
+                        const float d = r * __builtin_fmaf(-n[k], dot, g[k]);
+                        g[k] = KIND == kMixed && is_v ? dy.at(k) : d;
+                    }
+                }
+                if (live) Row::store(a.out[0] + at + mine_at, g);
+            };
+            switch (kind_of(a, head0, HEADS)) {
+            case kQuery: work(std::integral_constant<Kind, kQuery>()); break;
+            case kKey: work(std::integral_constant<Kind, kKey>()); break;
+            case kValue: work(std::integral_constant<Kind, kValue>()); break;
+            default: work(std::integral_constant<Kind, kMixed>()); break;
             }
-            if (live) Row::store(a.out[0] + at, d);
         }
         __syncthreads();
     }
@@ -315,7 +378,7 @@ struct NormCall {
 };
 
 template <class Row, int LANES, int NSRC>
-static hipError_t launch_norm(const NormCall &c, hipStream_t stream)
+static hipError_t launch_norm(NormCall &c, hipStream_t stream)
 {
     NormArgs<NSRC> a = {};
     for (int i = 0; i < NSRC; ++i) a.src[i] = static_cast<const char *>(c.bufs[i]);
@@ -333,17 +396,19 @@ static hipError_t launch_norm(const NormCall &c, hipStream_t stream)
     a.interleaved = c.interleaved;
     a.tokens_per_wg = c.tokens_per_wg;
     a.eps = c.eps;
-    if (c.backward)
+    if (c.backward) { // a partial row from each workgroup
+        const unsigned most = static_cast<unsigned>(compute_units()) * kGradPerUnit<Row, NSRC>;
+        c.workgroups = c.workgroups < most ? c.workgroups : most;
         hipLaunchKernelGGL((qk_norm_rope_backward_kernel<Row, LANES, NSRC>), dim3(c.workgroups), dim3(kNormBlock), 0,
                            stream, a);
-    else
+    } else
         hipLaunchKernelGGL((qk_norm_rope_kernel<Row, LANES, NSRC>), dim3(c.workgroups), dim3(kNormBlock), 0, stream,
                            a);
     return hipGetLastError();
 }
 
 template <class Row, int LANES>
-static hipError_t launch_norm_nsrc(const NormCall &c, hipStream_t stream)
+static hipError_t launch_norm_nsrc(NormCall &c, hipStream_t stream)
 {
     switch (c.world) {
     case 1: return launch_norm<Row, LANES, 1>(c, stream);
@@ -359,7 +424,7 @@ static hipError_t launch_norm_nsrc(const NormCall &c, hipStream_t stream)
 }
 
 template <class Row>
-static hipError_t launch_norm_dim(const NormCall &c, hipStream_t stream)
+static hipError_t launch_norm_dim(NormCall &c, hipStream_t stream)
 {
     switch (c.dim) {
     case 64: return launch_norm_nsrc<Row, 8>(c, stream);
@@ -377,12 +442,9 @@ static int norm_tokens_per_wg(const NormCall &c)
     return groups >= kNormWaves ? 1 : (groups >= 2 ? 2 : 4);
 }
 
-// Workgroups of the backward pass: each leaves one partial row.
-static unsigned backward_workgroups(const NormCall &c)
+static unsigned norm_workgroups(const NormCall &c)
 {
-    const size_t need = (c.tokens + c.tokens_per_wg - 1) / c.tokens_per_wg;
-    const size_t most = static_cast<size_t>(compute_units()) * 4;
-    return static_cast<unsigned>(need < most ? need : most);
+    return static_cast<unsigned>((c.tokens + c.tokens_per_wg - 1) / c.tokens_per_wg);
 }
 
 static int check_norm(const NormCall &c, int dtype)
@@ -434,7 +496,7 @@ extern "C" int tccl_qk_norm_rope(const void *const *bufs, int world, void *q_out
     if (const int rc = check_norm(c, dtype)) return rc;
     if (tokens == 0) return TCCL_OK;
     c.tokens_per_wg = norm_tokens_per_wg(c);
-    c.workgroups = static_cast<unsigned>((tokens + c.tokens_per_wg - 1) / c.tokens_per_wg);
+    c.workgroups = norm_workgroups(c);
     hipStream_t s = static_cast<hipStream_t>(stream);
     return hip_code(dtype == TCCL_BF16 ? launch_norm_dim<Bf16Row>(c, s) : launch_norm_dim<F32Row>(c, s));
 }
@@ -442,7 +504,7 @@ extern "C" int tccl_qk_norm_rope(const void *const *bufs, int world, void *q_out
 extern "C" size_t tccl_qk_norm_rope_backward_workspace(int head_dim)
 {
     if (head_dim != 64 && head_dim != 128 && head_dim != 256) return 0;
-    return static_cast<size_t>(compute_units()) * 4 * 2 * head_dim * sizeof(float);
+    return static_cast<size_t>(compute_units()) * kMostGradPerUnit * 2 * head_dim * sizeof(float);
 }
 
 extern "C" int tccl_qk_norm_rope_backward(const void *const *bufs, int world, const void *dq, const void *dk,
@@ -473,7 +535,7 @@ extern "C" int tccl_qk_norm_rope_backward(const void *const *bufs, int world, co
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (tokens > 0) {
         c.tokens_per_wg = norm_tokens_per_wg(c);
-        c.workgroups = backward_workgroups(c);
+        c.workgroups = norm_workgroups(c);
         const hipError_t e = dtype == TCCL_BF16 ? launch_norm_dim<Bf16Row>(c, s) : launch_norm_dim<F32Row>(c, s);
         if (e != hipSuccess) return hip_code(e);
     }

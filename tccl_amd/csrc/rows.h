@@ -76,7 +76,7 @@ __device__ __forceinline__ float dpp(float x)
     const int i = __builtin_bit_cast(int, x);
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(i, i, CTRL, 0xF, 0xF, false));
 }
-constexpr int kDppXor1 = 0xB1, kDppXor2 = 0x4E, kDppHalfMirror = 0x141, kDppMirror = 0x140;
+constexpr int kDppXor1 = 0xB1, kDppXor2 = 0x4E, kDppHalfMirror = 0x141, kDppMirror = 0x140, kDppRotate8 = 0x128;
 
 struct AddOp {
     static __device__ __forceinline__ float of(float a, float b) { return a + b; }
