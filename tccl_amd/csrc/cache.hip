@@ -101,34 +101,47 @@ __device__ __forceinline__ void turn_group(const uint32_t (&in)[16], uint32_t (&
     }
 }
 
-// Largest finite magnitude of a lane's elements, as fp32 bits (order-preserving for magnitudes).
-__device__ __forceinline__ float finite_magnitude(const float *x)
+// A row with infinities or NaN: its scale comes from the largest finite magnitude, what is not finite becomes NaN.
+template <class Row, int LANES>
+__device__ __forceinline__ u32x2 codes_of_special_row(Row x, uint32_t &scale)
 {
-    float m = 0.0f;
+    constexpr uint32_t NOT_FINITE = 0x7F800000u;
+    uint32_t largest = 0, nan = 0;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-        const float a = __builtin_fabsf(x[k]);
-        m = fmaxf(m, __builtin_isfinite(a) ? a : 0.0f);
+        const uint32_t u = f32_to_bits(x.at(k)) & 0x7FFFFFFFu;
+        if (u >= NOT_FINITE)
+            nan |= 1u << k;
+        else
+            largest = largest > u ? largest : u;
     }
-    return m;
+    scale = scale_byte(f32_to_bits(reduce_row<MaxOp, LANES>(bits_to_f32(largest))));
+    u32x2 r = x.codes(scale_of(scale));
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+        if (nan & (1u << k)) r[k >> 2] |= 0x7Fu << (8 * (k & 3));
+    return r;
 }
 
 // Eight elements as they are stored: four dwords of bf16, or two of codes (and the row's scale byte).
-template <class Store, int LANES>
-__device__ __forceinline__ void encode(const float *x, char *to, uint32_t &scale)
+template <class Row, class Store, int LANES>
+__device__ __forceinline__ void encode(const Row &x, char *to, uint32_t &scale)
 {
     if constexpr (Store::kScaled) {
-        scale = scale_byte(f32_to_bits(reduce_row<MaxOp, LANES>(finite_magnitude(x))));
-        const float f = inverse_scale_of(scale);
+        const uint32_t m = x.magnitude();
         u32x2 code;
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const uint32_t half = pack_e4m3<false>(x[4 * k] * f, x[4 * k + 1] * f, 0);
-            code[k] = pack_e4m3<true>(x[4 * k + 2] * f, x[4 * k + 3] * f, half);
+        if (__any(m >= 0x7F800000u)) {
+            code = codes_of_special_row<Row, LANES>(x, scale);
+        } else {
+            scale = scale_byte(f32_to_bits(reduce_row<MaxOp, LANES>(bits_to_f32(m))));
+            code = x.codes(scale_of(scale));
         }
         if (to != nullptr) *reinterpret_cast<u32x2 *>(to) = code;
-    } else {
-        if (to != nullptr) Bf16Row::store(to, x);
+    } else if (to != nullptr) {
+        float f[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) f[k] = x.at(k);
+        Bf16Row::store(to, f);
     }
 }
 
@@ -164,18 +177,11 @@ cache_write_kernel(CacheArgs a)
         if (t >= TOKENS) break; // whole waves
         char *const block = runs.block[t];
         const int place = runs.place[t];
-        float x[8];
         uint32_t k_scale = 0, v_scale = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = k[i].at(j);
-        encode<Store, LANES>(x,
-                             block == nullptr ? nullptr
-                                              : block + ((static_cast<size_t>(place >> 4) * (D / GROUP) + p * 8 / GROUP) * 16 +
-                                                         (place & 15)) * 16 + (p * 8 % GROUP) * BYTES,
-                             k_scale);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = v[i].at(j);
-        encode<Store, LANES>(x, values + (t * D + p * 8) * BYTES, v_scale);
+        const size_t chunk = static_cast<size_t>(place >> 4) * (D / GROUP) + p * 8 / GROUP;
+        encode<Row, Store, LANES>(
+            k[i], block == nullptr ? nullptr : block + (chunk * 16 + (place & 15)) * 16 + (p * 8 % GROUP) * BYTES, k_scale);
+        encode<Row, Store, LANES>(v[i], values + (t * D + p * 8) * BYTES, v_scale);
         if (Store::kScaled && block != nullptr && p == 0) {
             block[scales_at + place] = static_cast<char>(k_scale);
             block[scales_at + page_size + place] = static_cast<char>(v_scale);

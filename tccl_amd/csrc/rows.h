@@ -7,6 +7,8 @@
 namespace tccl {
 
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+typedef int16_t s16x2 __attribute__((ext_vector_type(2)));
 
 struct PoolTable {
     char *p[TCCL_MAX_WORLD];
@@ -25,6 +27,28 @@ struct Bf16Row {
     __device__ __forceinline__ float at(int k) const
     {
         return bits_to_f32((k & 1) ? raw[k >> 1] & 0xFFFF0000u : raw[k >> 1] << 16);
+    }
+    // the largest magnitude's fp32 bits (integers in the order of the magnitudes; infinity and NaN above all)
+    __device__ __forceinline__ uint32_t magnitude() const
+    {
+        u16x2 m = __builtin_bit_cast(u16x2, raw[0] & 0x7FFF7FFFu);
+#pragma unroll
+        for (int i = 1; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, raw[i] & 0x7FFF7FFFu));
+        return static_cast<uint32_t>(m.x > m.y ? m.x : m.y) << 16;
+    }
+    // the eight elements divided by a power of two as e4m3 codes, rounded to nearest even; all finite
+    __device__ __forceinline__ u32x2 codes(float scale) const
+    {
+        u32x2 r;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            s16x2 c = {0, 0};
+            const uint32_t low = raw[2 * i], high = raw[2 * i + 1];
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(c, __builtin_bit_cast(bf16x2, low), scale, false);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(c, __builtin_bit_cast(bf16x2, high), scale, true);
+            r[i] = __builtin_bit_cast(uint32_t, c);
+        }
+        return r;
     }
     static __device__ __forceinline__ void store(char *p, const float *x)
     {
@@ -48,6 +72,28 @@ struct F32Row {
     }
     __device__ __forceinline__ void zero() { raw[0] = raw[1] = u32x4{0, 0, 0, 0}; }
     __device__ __forceinline__ float at(int k) const { return bits_to_f32(raw[k >> 2][k & 3]); }
+    __device__ __forceinline__ uint32_t magnitude() const
+    {
+        uint32_t m = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const uint32_t u = raw[k >> 2][k & 3] & 0x7FFFFFFFu;
+            m = m > u ? m : u;
+        }
+        return m;
+    }
+    __device__ __forceinline__ u32x2 codes(float scale) const
+    {
+        u32x2 r;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            s16x2 c = {0, 0};
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c, at(4 * i), at(4 * i + 1), scale, false);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c, at(4 * i + 2), at(4 * i + 3), scale, true);
+            r[i] = __builtin_bit_cast(uint32_t, c);
+        }
+        return r;
+    }
     static __device__ __forceinline__ void store(char *p, const float *x)
     {
 #pragma unroll
@@ -153,18 +199,6 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t largest_bits)
     return static_cast<uint32_t>((e < kLeastExponent ? kLeastExponent : e) + 127);
 }
 __device__ __forceinline__ float scale_of(uint32_t byte) { return bits_to_f32(byte << 23); }
-__device__ __forceinline__ float inverse_scale_of(uint32_t byte) { return bits_to_f32((254u - byte) << 23); }
-
-// Two fp32 -> two e4m3 codes (round to nearest even) in the low or high half of `old`.  Infinities and NaN
-// become the NaN code.
-template <bool HIGH>
-__device__ __forceinline__ uint32_t pack_e4m3(float a, float b, uint32_t old)
-{
-    const float nan = __builtin_nanf("");
-    a = __builtin_isfinite(a) ? a : nan;
-    b = __builtin_isfinite(b) ? b : nan;
-    return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(a, b, static_cast<int>(old), HIGH));
-}
 
 // Where a slot (page * page_size + place in the page) of head h lies; nullptr outside the pool.
 struct PoolShape {
