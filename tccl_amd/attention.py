@@ -130,19 +130,20 @@ def qk_norm_rope(tensor: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.T
     lib = _lib.load()
     with _collective():
         tokens = tensor.shape[0]
-        outs = [tensor.new_empty((tokens, n, dim)) for n in heads]
+        q, k, v = (tensor.new_empty((tokens, q_heads, dim)), tensor.new_empty((tokens, k_heads, dim)),
+                   tensor.new_empty((tokens, v_heads, dim)))
         if tokens == 0:                # (an empty view has no address to find a group by)
-            return outs[0], outs[1], outs[2]
+            return q, k, v
         symm = rendezvous(tensor)
         _refuse_remote(symm.group, "qk_norm_rope")
         symm.group.check_signals()
         with _on(tensor.device):
-            rc = lib.tccl_qk_norm_rope(symm.buffer_ptrs_host, symm.world_size, *(o.data_ptr() or None for o in outs),
-                                       q_weight.data_ptr(), k_weight.data_ptr(), positions.data_ptr(),
-                                       inv_freq.data_ptr() or None, tokens, *heads, dim, rotary, int(interleaved), eps,
-                                       dtype, _stream(tensor.device))
+            rc = lib.tccl_qk_norm_rope(symm.buffer_ptrs_host, symm.world_size, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                       q_weight.data_ptr(), k_weight.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(),
+                                       tokens, q_heads, k_heads, v_heads, dim, rotary, interleaved, eps, dtype,
+                                       _stream(tensor.device))
         _lib.check("tccl_qk_norm_rope", rc)
-    return outs[0], outs[1], outs[2]
+    return q, k, v
 
 
 def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor, dv: torch.Tensor, tensor: torch.Tensor,
@@ -178,9 +179,9 @@ def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor, dv: torch.Tensor, 
             workspace = tensor.new_empty(nbytes, dtype=torch.uint8)
             first = dweights.data_ptr()
             rc = lib.tccl_qk_norm_rope_backward(
-                symm.buffer_ptrs_host, symm.world_size, *(g.data_ptr() or None for g in (dq, dk, dv)), q_weight.data_ptr(),
-                k_weight.data_ptr(), positions.data_ptr(), inv_freq.data_ptr() or None, dx.data_ptr(), first, first + 4 * dim,
-                workspace.data_ptr(), nbytes, tokens, *heads, dim, rotary, int(interleaved), eps, dtype, _stream(device))
+                symm.buffer_ptrs_host, symm.world_size, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), q_weight.data_ptr(),
+                k_weight.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), dx.data_ptr(), first, first + 4 * dim,
+                workspace.data_ptr(), nbytes, tokens, *heads, dim, rotary, interleaved, eps, dtype, _stream(device))
         _lib.check("tccl_qk_norm_rope_backward", rc)
     return (dx, *dweights.unbind(0))
 
@@ -328,7 +329,7 @@ def decode_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tenso
                 nbytes = _attention_workspace(batch, q_heads, cache.kv_heads, dim, most, device)
                 workspace = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
                 rc = _lib.load().tccl_decode_attention(
-                    cache._ref, q.data_ptr(), *q_strides, page_table.data_ptr() or None, row, lengths.data_ptr(), out.data_ptr(),
+                    cache._ref, q.data_ptr(), *q_strides, page_table.data_ptr(), row, lengths.data_ptr(), out.data_ptr(),
                     lse.data_ptr() if lse is not None else None, workspace.data_ptr() if nbytes else None, nbytes, batch, q_heads,
                     most, scale, _stream(device))
             _lib.check("tccl_decode_attention", rc)
