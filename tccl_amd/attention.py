@@ -232,9 +232,9 @@ def cache_write(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, slots: torc
     (padding); the slots of one call must differ from each other."""
     dtype = _sum_dtype(k)
     tokens = slots.numel()
-    for t, name in ((k, "k"), (v, "v")):
-        if t.shape != cache._rows(tokens) or t.dtype != k.dtype or t.device != cache.device:
-            raise ValueError(f"{name} must be a {k.dtype} tensor of shape {cache._rows(tokens)} on {cache.device}")
+    rows, device = (tokens, cache.kv_heads, cache.head_dim), cache.device
+    if k.shape != rows or v.shape != rows or v.dtype != k.dtype or k.device != device or v.device != device:
+        raise ValueError(f"k and v must be tensors of one dtype, of shape {rows}, on {device}")
     strides = _heads_first(k, "k") + _heads_first(v, "v")
     _integers(slots, torch.int64, (tokens,), cache.device, "slots")
     if tokens == 0:
@@ -254,8 +254,7 @@ def cache_read(cache: PagedCache, slots: torch.Tensor, *, dtype: torch.dtype = t
     _integers(slots, torch.int64, (tokens,), cache.device, "slots")
     _need(dtype in (torch.bfloat16, torch.float32), "cache_read returns bfloat16 or float32")
     if out is None:
-        rows = cache._rows(tokens)
-        k, v = slots.new_empty(rows, dtype=dtype), slots.new_empty(rows, dtype=dtype)
+        k, v = slots.new_empty((2, tokens, cache.kv_heads, cache.head_dim), dtype=dtype).unbind(0)     # one allocation
     else:
         k, v = out
         for t, name in ((k, "out[0]"), (v, "out[1]")):
