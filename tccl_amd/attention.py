@@ -77,6 +77,10 @@ def _heads_first(t: torch.Tensor, name: str) -> Tuple[int, int]:
     if t.numel() == 0:
         return 0, 0
     token, head, element = t.stride()
+    if t.shape[0] == 1:                # (the stride of a dimension of one means nothing)
+        token = 0
+    if t.shape[1] == 1:
+        head = 0
     vec = 16 // t.element_size()
     if element != 1 or token % vec or head % vec or t.data_ptr() % 16:
         raise ValueError(f"{name}: rows of head_dim elements must be contiguous and start at multiples of 16 bytes")

@@ -405,9 +405,9 @@ decode_attention_kernel(AttnArgs a)
         row_begin = row_end;
         if (++hg == a.head_groups) {
             hg = 0;
-            if (unit < stop)
+            if (unit < stop) // there is a next row with tokens
                 do length = sequence_length(a, ++b);
-                while (length == 0);
+                while (length == 0 && b + 1 < a.batch);
         }
     }
 }

@@ -487,6 +487,10 @@ def test_decode_attention_strides_and_outputs():
         check_attention(out, lse, q, keys, values)
     only = tccl_amd.decode_attention(q.to(DEV), cache, table, n)
     assert_bit_equal(only, out, "without lse")
+    # a dimension of one may have any stride
+    odd = torch.zeros(8 * 64, dtype=BF16, device=DEV).as_strided((1, 8, 64), (3, 64, 1)).copy_(q[2:].to(DEV))
+    alone = tccl_amd.decode_attention(odd, cache, table[2:], n[2:])
+    check_attention(alone, None, q[2:], keys[2:], values[2:])
     # one query row for every sequence
     one = q[:1].to(DEV).expand(3, 8, 64)
     check_attention(tccl_amd.decode_attention(one, cache, table, n), None, q[:1].expand(3, 8, 64), keys, values)
