@@ -237,13 +237,12 @@ decode_attention_kernel(AttnArgs a)
                 const int at = start + (m >> 2) * TOKENS, p = (at >> shift) - first_page;
                 const char *kb = p < npages ? pages[p] : nullptr;
                 kb = kb != nullptr ? kb : safe;
+                const int in = (at & (page_size - 1)) + (m & 3);
+                const char *row = kb + static_cast<size_t>(in >> 4) * (D / Store::kChunk) * 256 + (in & 15) * 16 + g * 256;
 #pragma unroll
-                for (int t = 0; t < TILES; ++t) {
-                    const int in = (at & (page_size - 1)) + 4 * t + (m & 3);
-                    const char *row = kb + static_cast<size_t>(in >> 4) * (D / Store::kChunk) * 256 + (in & 15) * 16;
+                for (int c = 0; c < KLOADS; ++c) // tiles innermost: they share cache lines
 #pragma unroll
-                    for (int c = 0; c < KLOADS; ++c) k[t][c] = load_vec<NT>(row + (c * 4 + g) * 256, 0);
-                }
+                    for (int t = 0; t < TILES; ++t) k[t][c] = load_vec<NT>(row + c * 1024 + t * 64, 0);
             };
             // values and scores: group g.  `live`: the tokens of it that count
             int live = 0;
