@@ -237,12 +237,15 @@ decode_attention_kernel(AttnArgs a)
                 const int at = start + (m >> 2) * TOKENS, p = (at >> shift) - first_page;
                 const char *kb = p < npages ? pages[p] : nullptr;
                 kb = kb != nullptr ? kb : safe;
-                const int in = (at & (page_size - 1)) + (m & 3);
-                const char *row = kb + static_cast<size_t>(in >> 4) * (D / Store::kChunk) * 256 + (in & 15) * 16 + g * 256;
+                const int in = at & (page_size - 1), first = key_row<Store>(in) + (m & 3);
+                const char *row = kb + static_cast<size_t>(in >> 4) * (D / Store::kChunk) * 256 + first * 16 + g * 256;
+                // token 4 t of a group is key_row(4 t) = 4 t rows (8 bits) or 8 t rows on.  Tiles innermost: they share cache
+                // lines in 8 bits
+                constexpr int TILE_BYTES = Store::kScaled ? 64 : 128;
 #pragma unroll
-                for (int c = 0; c < KLOADS; ++c) // tiles innermost: they share cache lines
+                for (int c = 0; c < KLOADS; ++c)
 #pragma unroll
-                    for (int t = 0; t < TILES; ++t) k[t][c] = load_vec<NT>(row + c * 1024 + t * 64, 0);
+                    for (int t = 0; t < TILES; ++t) k[t][c] = load_vec<NT>(row + c * 1024 + t * TILE_BYTES, 0);
             };
             // values and scores: group g.  `live`: the tokens of it that count
             int live = 0;

@@ -180,7 +180,7 @@ cache_write_kernel(CacheArgs a)
         uint32_t k_scale = 0, v_scale = 0;
         const size_t chunk = static_cast<size_t>(place >> 4) * (D / GROUP) + p * 8 / GROUP;
         encode<Row, Store, LANES>(
-            k[i], block == nullptr ? nullptr : block + (chunk * 16 + (place & 15)) * 16 + (p * 8 % GROUP) * BYTES, k_scale);
+            k[i], block == nullptr ? nullptr : block + (chunk * 16 + key_row<Store>(place)) * 16 + (p * 8 % GROUP) * BYTES, k_scale);
         encode<Row, Store, LANES>(v[i], values + (t * D + p * 8) * BYTES, v_scale);
         if (Store::kScaled && block != nullptr && p == 0) {
             block[scales_at + place] = static_cast<char>(k_scale);
@@ -292,7 +292,7 @@ cache_read_kernel(CacheArgs a)
         const char *const block = runs.block[t];
         const int place = runs.place[t];
         if (block == nullptr) continue;
-        k[i] = load_vec<false>(block, (static_cast<size_t>(place >> 4) * CHUNKS + c) * 16 + (place & 15));
+        k[i] = load_vec<false>(block, (static_cast<size_t>(place >> 4) * CHUNKS + c) * 16 + key_row<Store>(place));
         if constexpr (Store::kScaled) k_scale[i] = static_cast<uint8_t>(block[scales_at + place]);
     }
     for (int item = threadIdx.x; item < runs.count * (D / 4); item += kCacheBlock) {

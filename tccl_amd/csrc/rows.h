@@ -163,8 +163,8 @@ __device__ __forceinline__ float reduce_row(float x)
 
 // ------------------------------------------------------------------ the paged cache's layout
 // One rank's buffer is [pages_per_rank][kv_heads] blocks; a block holds one head of one page:
-//   K        tiles of 16 tokens, each [head_dim / kKChunk][16 tokens][kKChunk elements]; a chunk is 16 bytes
-//   V        groups of kVTokens tokens, each [head_dim][kVTokens tokens]; again 16 bytes per dim
+//   K        tiles of 16 tokens, each [head_dim / kChunk][16 tokens, see key_row][kChunk elements]; a chunk is 16 bytes
+//   V        groups of kChunk tokens, each [head_dim][kChunk tokens]; again 16 bytes per dim
 //   K and V exponents, one byte (exponent + 127) per token each (8-bit storage only)
 // A wave's 16-byte loads of it are the operands of the attention's matrix instructions as they stand:
 // keys with their dims along the contraction, values with their tokens along it.
@@ -178,6 +178,14 @@ struct E4m3Store {
     static constexpr int kChunk = 16;
     static constexpr bool kScaled = true;
 };
+
+// A token's row in its K tile.  An attention load takes four tokens of each of two 8-token groups (bf16): they lie side
+// by side, a whole 128-byte line.
+template <class Store>
+__device__ __forceinline__ int key_row(int place)
+{
+    return Store::kScaled ? place & 15 : (place & 4) << 1 | (place & 8) >> 1 | (place & 3);
+}
 
 template <class Store>
 __host__ __device__ constexpr size_t cache_block_bytes(int page_size, int dim)
