@@ -269,8 +269,9 @@ template <class Row, class Store, int LANES, int TOKENS>
 __global__ void __launch_bounds__(kCacheBlock)
 cache_read_kernel(CacheArgs a)
 {
-    constexpr int D = 8 * LANES, BYTES = Store::kBytes, GROUP = Store::kChunk, CHUNKS = D / GROUP;
-    constexpr int ROUNDS = (TOKENS * CHUNKS + kCacheBlock - 1) / kCacheBlock;
+    constexpr int D = 8 * LANES, BYTES = Store::kBytes, GROUP = Store::kChunk, CODES = 2 * BYTES;
+    constexpr int ROUNDS = (TOKENS * LANES + kCacheBlock - 1) / kCacheBlock;
+    typedef uint32_t codes_t __attribute__((ext_vector_type(CODES)));
     __shared__ Runs<TOKENS> runs;
     const int h = blockIdx.y;
     const size_t begin = static_cast<size_t>(blockIdx.x) * TOKENS;
@@ -281,18 +282,19 @@ cache_read_kernel(CacheArgs a)
     if (threadIdx.x < 64) find_runs<GROUP, TOKENS>(a, begin, h, runs);
     __syncthreads();
     const int here = a.tokens - begin < TOKENS ? static_cast<int>(a.tokens - begin) : TOKENS;
-    u32x4 k[ROUNDS];
+    codes_t k[ROUNDS]; // eight elements of a row per lane, as the stores want them
     uint32_t k_scale[ROUNDS];
 #pragma unroll
     for (int i = 0; i < ROUNDS; ++i) {
-        const int t = (threadIdx.x + i * kCacheBlock) / CHUNKS, c = (threadIdx.x + i * kCacheBlock) % CHUNKS;
-        k[i] = u32x4{0, 0, 0, 0};
+        const int t = (threadIdx.x + i * kCacheBlock) / LANES, p = (threadIdx.x + i * kCacheBlock) % LANES;
+        k[i] = codes_t(0);
         k_scale[i] = 0;
         if (t >= here) continue;
         const char *const block = runs.block[t];
         const int place = runs.place[t];
         if (block == nullptr) continue;
-        k[i] = load_vec<false>(block, (static_cast<size_t>(place >> 4) * CHUNKS + c) * 16 + key_row<Store>(place));
+        const size_t chunk = static_cast<size_t>(place >> 4) * (D / GROUP) + p * 8 / GROUP;
+        k[i] = *reinterpret_cast<const codes_t *>(block + (chunk * 16 + key_row<Store>(place)) * 16 + (p * 8 % GROUP) * BYTES);
         if constexpr (Store::kScaled) k_scale[i] = static_cast<uint8_t>(block[scales_at + place]);
     }
     for (int item = threadIdx.x; item < runs.count * (D / 4); item += kCacheBlock) {
@@ -321,21 +323,18 @@ cache_read_kernel(CacheArgs a)
     }
 #pragma unroll
     for (int i = 0; i < ROUNDS; ++i) {
-        const int t = (threadIdx.x + i * kCacheBlock) / CHUNKS, c = (threadIdx.x + i * kCacheBlock) % CHUNKS;
+        const int t = (threadIdx.x + i * kCacheBlock) / LANES, p = (threadIdx.x + i * kCacheBlock) % LANES;
         if (t >= here) continue;
-        const uint32_t code[4] = {k[i][0], k[i][1], k[i][2], k[i][3]};
-        char *const out = a.k_out + to + t * token_bytes + c * GROUP * Row::kElemBytes;
+        uint32_t code[CODES];
 #pragma unroll
-        for (int part = 0; part < GROUP / 8; ++part) {
-            float x[8];
-            decode<Store, 8>(code + 2 * part, scale_of(k_scale[i]), x);
-            Row::store(out + part * 8 * Row::kElemBytes, x);
-        }
+        for (int w = 0; w < CODES; ++w) code[w] = k[i][w];
+        const size_t at = to + t * token_bytes + p * 8 * Row::kElemBytes;
+        float x[8];
+        decode<Store, 8>(code, scale_of(k_scale[i]), x);
+        Row::store(a.k_out + at, x);
         if (runs.block[t] == nullptr) { // no run: the token's values are zeros as well
-            char *const v_out = a.v_out + to + t * token_bytes + c * GROUP * Row::kElemBytes;
             const float zeros[8] = {};
-#pragma unroll
-            for (int part = 0; part < GROUP / 8; ++part) Row::store(v_out + part * 8 * Row::kElemBytes, zeros);
+            Row::store(a.v_out + at, zeros);
         }
     }
 }
