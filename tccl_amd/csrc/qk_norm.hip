@@ -11,6 +11,8 @@
 // elements, so a wave works on 512 consecutive elements (four heads of 128) with one 16-byte load per
 // source; the mean is a reduction over head_dim / 8 lanes in registers.  Angles are formed in fp64 turns
 // (fp32 would lose the fraction of a far position's angle) once per token by the workgroup, into LDS.
+// Measured: forward, 4,099 tokens of 48 heads of 128, 8 bf16 sources 78 us, 5.8 TB/s; 8,191 tokens of 20 heads of 256, one
+// fp32 source 63 us, 5.3 TB/s read and written; backward, 8,192 tokens of 48 heads of 128, one bf16 source 52 us, 5.6 TB/s.
 #include <type_traits>
 
 #include "host.h"
@@ -434,7 +436,9 @@ static hipError_t launch_norm_dim(NormCall &c, hipStream_t stream)
     }
 }
 
-// Tokens a workgroup takes at once: where a token has fewer than four waves' worth of heads, more tokens.
+// Tokens a workgroup takes at once: where a token has fewer than four waves' worth of heads, more tokens.  8,192 tokens
+// of three heads of 64, forward and backward: 8.7 and 11.7 us with four, 13.2 and 19.0 with one; of six heads of 128
+// 15.6 and 17.0 with two, 19.6 and 22.6 with one.
 static int norm_tokens_per_wg(const NormCall &c)
 {
     const int per_wave = 512 / c.dim;
