@@ -25,7 +25,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 constexpr int kAttnBlock = 256;
 constexpr int kAttnWaves = 4;
 constexpr int kPiecePages = 512;  // page addresses a workgroup looks up at once
-constexpr int kSharedBatch = 4096; // most sequences whose tokens are dealt out evenly
+constexpr size_t kBatch = 4096;  // sequences of a launch at most: every workgroup adds their lengths up
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
 struct AttnArgs {
@@ -602,8 +602,7 @@ struct AttnPlan {
 // and no second launch instead
 //   - where no sequence has over 512 tokens: 32 x 500 tokens, 8 key heads 15.4 us against 19.5;
 //   - where the rows alone fill the GPU eight times and none is so long that the last one would be waited for:
-//     512 x 500 tokens 123 us against 163, 256 x 1,000 126 against 133, but 128 x 2,000 136 against 126;
-//   - where dealing out would take too long in each workgroup (over 4,096 sequences).
+//     512 x 500 tokens 123 us against 163, 256 x 1,000 126 against 133, but 128 x 2,000 136 against 126.
 static AttnPlan plan_attention(size_t batch, int q_heads, int kv_heads, int head_dim, int most)
 {
     AttnPlan p = {};
@@ -612,15 +611,22 @@ static AttnPlan plan_attention(size_t batch, int q_heads, int kv_heads, int head
     p.head_groups = kv_heads * ((blocks + p.blocks_per_wg - 1) / p.blocks_per_wg);
     const size_t rows = batch * p.head_groups, units = compute_units();
     const size_t most_units = rows * ((static_cast<size_t>(most) + 127) / 128); // a unit is 128 or 256 tokens
-    if (most <= 512 || (rows >= 8 * units && most <= 2048) || batch > kSharedBatch ||
-        most_units >= (static_cast<size_t>(1) << 31))
-        return p;
+    if (most <= 512 || (rows >= 8 * units && most <= 2048) || most_units >= (static_cast<size_t>(1) << 31)) return p;
     const size_t at_once = units * (head_dim == 256 ? 1 : 2), wgs = at_once < most_units ? at_once : most_units;
     p.workgroups = static_cast<int>(wgs);
     p.part_floats = 2 * wgs * 16 * p.blocks_per_wg * head_dim;
     p.span_bytes = rows * sizeof(int2);
     p.workspace = p.part_floats * sizeof(float) + p.part_floats / head_dim * 2 * sizeof(float) + p.span_bytes;
     return p;
+}
+
+// What the launches of a batch need, one after the other: all but the last have kBatch sequences.
+static size_t attention_workspace(size_t batch, int q_heads, int kv_heads, int head_dim, int most)
+{
+    const size_t whole = batch < kBatch ? batch : kBatch, last = batch % kBatch;
+    const size_t a = plan_attention(whole, q_heads, kv_heads, head_dim, most).workspace;
+    const size_t b = plan_attention(last, q_heads, kv_heads, head_dim, most).workspace;
+    return a > b ? a : b;
 }
 
 template <class Store, int D>
@@ -673,7 +679,7 @@ using namespace tccl;
 extern "C" size_t tccl_decode_attention_workspace(size_t batch, int q_heads, int kv_heads, int head_dim, int max_tokens)
 {
     if (check_attention_shape(batch, q_heads, kv_heads, max_tokens) != TCCL_OK) return 0;
-    return plan_attention(batch, q_heads, kv_heads, head_dim, max_tokens).workspace;
+    return attention_workspace(batch, q_heads, kv_heads, head_dim, max_tokens);
 }
 
 extern "C" int tccl_decode_attention(const tccl_paged_cache *cache, const void *q, size_t q_batch_stride,
@@ -692,30 +698,36 @@ extern "C" int tccl_decode_attention(const tccl_paged_cache *cache, const void *
     if (!aligned16(q) || !aligned16(out) || !aligned16(workspace) || (a.q_batch | a.q_head) % kVecBytes != 0)
         return TCCL_EALIGN;
     if (batch == 0) return TCCL_OK;
-    const AttnPlan plan = plan_attention(batch, q_heads, cache->kv_heads, cache->head_dim, max_tokens);
-    if (plan.workspace > 0 && (workspace == nullptr || workspace_bytes < plan.workspace)) return TCCL_ESCRATCH;
-    if (!fits_launch(plan.workgroups > 0 ? batch * q_heads : batch * plan.head_groups, kAttnBlock)) return TCCL_EINVAL;
-    a.q = static_cast<const char *>(q);
-    a.table = page_table;
+    const size_t need = attention_workspace(batch, q_heads, cache->kv_heads, cache->head_dim, max_tokens);
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return TCCL_ESCRATCH;
+    if (!fits_launch((batch < kBatch ? batch : kBatch) * q_heads, kAttnBlock)) return TCCL_EINVAL;
     a.table_row = page_table_stride;
-    a.lengths = lengths;
-    a.out = static_cast<char *>(out);
-    a.lse = lse;
-    // the workspace: partial outputs, their maxima and sums, the rows' spans
-    a.part_o = static_cast<float *>(workspace);
-    a.part_ml = a.part_o + plan.part_floats;
-    a.spans = reinterpret_cast<int2 *>(a.part_ml + plan.part_floats / cache->head_dim * 2);
-    a.batch = static_cast<int>(batch);
     a.q_heads = q_heads;
     a.group = q_heads / cache->kv_heads;
-    a.blocks_per_wg = plan.blocks_per_wg;
-    a.head_groups = plan.head_groups;
     a.most = max_tokens;
-    a.workgroups = plan.workgroups;
     a.scale = scale * kLog2e;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    return hip_code(cache->dtype == TCCL_E4M3 ? launch_attention_dim<E4m3Store>(a, cache->head_dim, s)
-                                              : launch_attention_dim<Bf16Store>(a, cache->head_dim, s));
+    for (size_t first = 0; first < batch; first += kBatch) {
+        const size_t here = batch - first < kBatch ? batch - first : kBatch;
+        const AttnPlan plan = plan_attention(here, q_heads, cache->kv_heads, cache->head_dim, max_tokens);
+        a.q = static_cast<const char *>(q) + first * a.q_batch;
+        a.table = page_table + first * page_table_stride;
+        a.lengths = lengths + first;
+        a.out = static_cast<char *>(out) + first * q_heads * cache->head_dim * 2;
+        a.lse = lse == nullptr ? nullptr : lse + first * q_heads;
+        // the workspace: partial outputs, their maxima and sums, the rows' spans
+        a.part_o = static_cast<float *>(workspace);
+        a.part_ml = a.part_o + plan.part_floats;
+        a.spans = reinterpret_cast<int2 *>(a.part_ml + plan.part_floats / cache->head_dim * 2);
+        a.batch = static_cast<int>(here);
+        a.blocks_per_wg = plan.blocks_per_wg;
+        a.head_groups = plan.head_groups;
+        a.workgroups = plan.workgroups;
+        const hipError_t e = cache->dtype == TCCL_E4M3 ? launch_attention_dim<E4m3Store>(a, cache->head_dim, s)
+                                                       : launch_attention_dim<Bf16Store>(a, cache->head_dim, s);
+        if (e != hipSuccess) return hip_code(e);
+    }
+    return TCCL_OK;
 }
 
 extern "C" int tccl_attention_all_reduce(const void *const *outs, const void *const *lses, int world, void *out,

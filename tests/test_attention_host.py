@@ -108,7 +108,9 @@ def test_attention_entry_points_check_their_arguments():
     assert attn(desc(page_size=20)) == EINVAL and attn(None) == EINVAL
     for kw in (dict(q=0x1008), dict(out=0x4008), dict(ws=0x6004), dict(strides=(512, 60)), dict(strides=(508, 64))):
         assert attn(desc(), **kw) == EALIGN, kw
-    assert attn(desc(kv_heads=64), batch=1 << 20, heads=64, most=64) == EINVAL   # more workgroups than one launch has
+    assert attn(desc(), batch=5000, heads=8192, most=64) == EINVAL               # more workgroups than one launch has
+    sizes = [lib.tccl_decode_attention_workspace(n, 8, 4, 64, 3000) for n in (1, 100, 4096, 4097, 9000)]
+    assert sizes[3] >= max(sizes[:3]) and sizes[4] == sizes[3] == sizes[2]        # launches of 4,096 share it
     need = lib.tccl_decode_attention_workspace(1, 8, 4, 64, 100_000)
     assert need > 0
     assert attn(desc(), batch=1, most=100_000) == ESCRATCH
