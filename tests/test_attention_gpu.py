@@ -363,7 +363,9 @@ def test_cache_without_tokens():
 
 def check_attention(out, lse, q, keys, values, scale=None, what=""):
     """out is one bf16 rounding of sum p v / sum p.  A score of D products is off by (D + 4) u sum |q k| scale; exp2 of it by twice
-    that, 4 u and u |score| of the base change; P as two bf16 terms by 2^-18; the sums over n tokens by (n / 4 + 64) u."""
+    that, 4 u and u |score| of the base change; P as two bf16 terms by 2^-18; the sums over n tokens by (n / 4 + 64) u.  A term that
+    is below the smallest normal number, 2^-126, may count as zero: P has two terms per token and sum p is at least 1 (the
+    maximum's own), so all of them together move the output by at most 2 n 2^-126."""
     want, want_lse = ref.attention(q, keys, values, scale)
     dim = q.shape[-1]
     scale = 1 / math.sqrt(dim) if scale is None else scale
@@ -378,7 +380,7 @@ def check_attention(out, lse, q, keys, values, scale=None, what=""):
             s = kk @ q[b, h].double() * scale
             ds = (dim + 4) * U * (kk.abs() @ q[b, h].double().abs() * abs(scale)).max() + 4 * U * s.abs().max()
             rel = 2 * ds + 2.0 ** -17 + (n / 4 + 80) * U
-            bound[b, h] = half_step(BF16) * want[b, h].abs() * (1 + 2.0 ** -7) + rel * (torch.softmax(s, 0) @ vv.abs())
+            bound[b, h] = half_step(BF16) * want[b, h].abs() * (1 + 2.0 ** -7) + rel * (torch.softmax(s, 0) @ vv.abs()) + 2 * n * 2.0 ** -126
             bound_lse[b, h] = 2 * ds + (n / 4 + 80) * U + 4 * U * want_lse[b, h].abs()
     within(out, want, bound, f"out {what}")
     if lse is not None:
@@ -459,6 +461,27 @@ def test_decode_attention_peaked_scores_and_scales(store):
     for scale in (None, 1.0, 0.01, -0.3, 0.0):
         out, lse = tccl_amd.decode_attention(q.to(DEV), cache, table, n, scale=scale, return_lse=True)
         check_attention(out, lse, q, keys, values, scale, what=f"scale {scale}")
+
+
+@pytest.mark.parametrize("store", [BF16, E4M3])
+@pytest.mark.parametrize("spread,scale", [(1e-20, None), (1e15, 1e-30), (1e-36, 1.0)])
+def test_decode_attention_tiny_and_huge_cached_values(store, spread, scale):
+    cache, table, n, q, keys, values, _ = filled(2, [300, 31], 8, 2, 64, 16, store, seed=5, spread=spread)
+    out, lse = tccl_amd.decode_attention(q.to(DEV), cache, table, n, scale=scale, return_lse=True)
+    check_attention(out, lse, q, keys, values, scale, what=f"values about {spread}")
+
+
+def test_decode_attention_nan_in_a_query_stays_in_its_head():
+    cache, table, n, q, keys, values, _ = filled(2, [700, 90], 12, 3, 64, 16, E4M3, seed=6)
+    q[0, 5, 9], q[1, 2, 0] = math.nan, math.inf
+    out, lse = (t.cpu() for t in tccl_amd.decode_attention(q.to(DEV), cache, table, n, return_lse=True))
+    bad = torch.zeros(2, 12, dtype=torch.bool)
+    bad[0, 5] = bad[1, 2] = True
+    assert torch.isnan(out[bad]).all() and torch.isnan(lse[0, 5])
+    fine = torch.where(bad[..., None], 0.0, q.double()).to(BF16)
+    clean, clean_lse = tccl_amd.decode_attention(fine.to(DEV), cache, table, n, return_lse=True)
+    assert_bit_equal(out[~bad], clean.cpu()[~bad], "the other heads")
+    assert_bit_equal(lse[~bad], clean_lse.cpu()[~bad], "the other heads' lse")
 
 
 def test_decode_attention_large_negative_scores_only():
