@@ -220,6 +220,7 @@ class PagedCache:
         nbytes = _lib.load().tccl_paged_cache_bytes(ctypes.byref(desc))
         # a group of its own, but not one that rendezvous finds: its buffers are no operand of a collective
         self.group = SymmGroup([torch.zeros(nbytes, dtype=torch.uint8, device=device) for _ in range(world_size)])
+        self.group.handles.clear()     # (they point back at the group: the buffers would outlive the cache until a collection)
         self.device = self.group.tensors[0].device
         for r, p in enumerate(self.group.buffer_ptrs):
             desc.bufs[r] = p

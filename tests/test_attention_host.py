@@ -1,10 +1,12 @@
 """The attention operators on a machine without a GPU: what their entry points and host wrappers refuse before
 anything is launched, the struct that crosses the ABI, and the 64-bit reference against differences."""
 import ctypes
+import gc
 import math
 import os
 import shutil
 import subprocess
+import weakref
 
 import pytest
 import torch
@@ -202,6 +204,13 @@ def test_paged_cache_refusals():
             tccl_amd.PagedCache(**{**good, **kw})
     cache = tccl_amd.PagedCache(**good)
     assert cache.pages == 6 and cache.slots == 96
+    gone = weakref.ref(cache.group.tensors[1])
+    gc.disable()
+    try:
+        cache = tccl_amd.PagedCache(**good)
+        assert gone() is None, "a dropped cache keeps its buffers until a garbage collection"
+    finally:
+        gc.enable()
     k, slots = torch.zeros(5, 2, 64), torch.arange(5)
     for bad in ((k[:4], k, slots), (k, k[:, :1], slots), (k, k.bfloat16(), slots), (k, k, slots.int()), (k, k, torch.arange(10)[::2]),
                 (k.transpose(1, 2).contiguous().transpose(1, 2), k, slots), (torch.zeros(5, 2, 65)[..., :64], k, slots),
