@@ -283,7 +283,9 @@ qk_norm_rope_backward_kernel(NormArgs<NSRC> a)
                 if constexpr (KIND != kValue) {
                     float n[8], dot = 0.0f;
                     sum_sources<Row, NSRC>(in, n);
-                    const float r = inverse_rms<LANES>(n, a.eps);
+                    // a lane without a head or token, or with a value head, holds zeros: where eps is 0 their root's inverse is
+                    // infinite and 0 times it NaN, so that n is made 0 by r and adds nothing to dw
+                    const float root = inverse_rms<LANES>(n, a.eps), r = live && !is_v ? root : 0.0f;
                     rotate<LANES, -1>(g, turn + local * (a.rotary >> 1), place, a.rotary, a.interleaved != 0);
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
@@ -291,7 +293,6 @@ qk_norm_rope_backward_kernel(NormArgs<NSRC> a)
                         const float gn = g[k] * n[k];
                         g[k] = g[k] * weight(k);
                         dot = __builtin_fmaf(g[k], n[k], dot);
-                        // a value head's (and a missing head's) x is zero here, and so is its gn
                         if constexpr (KIND == kMixed) {
                             dw[0][k] = dw[0][k] + (is_q ? gn : 0.0f);
                             dw[1][k] = dw[1][k] + (is_q || is_v ? 0.0f : gn);

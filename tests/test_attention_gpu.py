@@ -157,6 +157,54 @@ def test_qk_norm_rope_backward(case):
         within(got[1 + i], want[1 + i], (chain + world + 64) * U * terms, name)
 
 
+def check_backward(got, parts, w, positions, inv_freq, grads, heads, eps, interleaved, per_lane):
+    """`per_lane`: how many terms of a weight's gradient a lane adds up at most.  The counts are those of
+    test_qk_norm_rope_backward; eps in the root makes every factor smaller, except that 1 / sqrt(mean x^2 + eps) then moves by
+    less than an error of x, which the bounds do not use."""
+    world, tokens, dim, dtype = len(parts), parts[0].shape[0], w[0].numel(), parts[0].dtype
+    want = ref.qk_norm_rope_grad(parts, grads, *w, positions, inv_freq, eps, interleaved)
+    x = sum(p.double() for p in parts).view(tokens, -1, dim)
+    absolute = sum(p.double().abs() for p in parts).view(tokens, -1, dim)
+    r = 1 / torch.sqrt(x.square().mean(-1, keepdim=True) + eps)
+    n = absolute * r
+    weight = torch.cat([torch.ones(tokens, heads[i], dim, dtype=torch.float64) * (w[i].double() if i < 2 else 1) for i in range(3)], 1)
+    g = 2 * row_max(torch.cat([t.double() for t in grads], 1))       # a rotated pair
+    m = r * g * row_max(weight) * (1 + row_max(n) ** 2) * (1 + row_max(n))
+    m[:, heads[0] + heads[1]:] = 0
+    dx, want_dx = got[0].view(tokens, -1, dim), want[0].view(tokens, -1, dim)
+    within(dx, want_dx, half_step(dtype) * want_dx.abs() * (1 + 2.0 ** -7) + (world + 56) * U * m, f"dx w{world} eps {eps}")
+    for i, name in enumerate(("dq_weight", "dk_weight")):
+        part = slice(0, heads[0]) if i == 0 else slice(heads[0], heads[0] + heads[1])
+        terms = (g[:, part] * n[:, part] * (1 + row_max(n[:, part]))).sum((0, 1))
+        within(got[1 + i], want[1 + i], (per_lane + 50 + world + 64) * U * terms, f"{name} eps {eps}")
+
+
+EPS_CASES = [
+    # world, tokens, heads, dim, rotary, interleaved, dtype: what of a wave has no work
+    (1, 5, (3, 1, 1), 64, 64, False, F32),       # the last workgroup has one token of four; heads of every kind in one wave
+    (2, 6, (3, 0, 0), 64, 32, True, BF16),        # query heads only, five places of eight without a head
+    (1, 7, (12, 0, 0), 64, 64, False, F32),       # two waves of heads per token, the second half empty, one token of two missing
+    (3, 9, (16, 3, 0), 128, 128, False, BF16),    # the keys' wave has one place without a head
+    (1, 3, (0, 5, 0), 256, 48, False, F32),
+    (2, 3, (2, 2, 3), 128, 0, False, F32),        # queries and keys fill a wave, the values' wave is cut
+    (1, 9, (8, 4, 1), 64, 16, True, BF16),        # keys, a value and empty places in one wave
+]
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-30, 1e-2, 100.0])
+@pytest.mark.parametrize("case", EPS_CASES, ids=lambda c: "-".join(str(x).replace("torch.", "") for x in c))
+def test_qk_norm_rope_any_eps_with_heads_and_tokens_missing(case, eps):
+    """Rows that are not zero have a norm and gradients for eps = 0 too; lanes without a head or a token add nothing to them."""
+    world, tokens, heads, dim, rotary, interleaved, dtype = case
+    parts, w, positions, inv_freq, grads = norm_inputs(world, tokens, heads, dim, rotary, dtype, seed=2)
+    group = world_of(parts)
+    dev = [t.to(DEV) for t in (*w, positions, inv_freq)]
+    got = tccl_amd.qk_norm_rope(group.tensor(0), *dev, heads[0], heads[1], eps=eps, interleaved=interleaved)
+    check_forward(got, parts, w, positions, inv_freq, heads, eps, interleaved)
+    got = tccl_amd.qk_norm_rope_backward(*(g.to(DEV) for g in grads), group.tensor(0), *dev, eps=eps, interleaved=interleaved)
+    check_backward(got, parts, w, positions, inv_freq, grads, heads, eps, interleaved, sum(heads))
+
+
 def test_qk_norm_rope_backward_against_differences():
     """<dx, d> and <dw, d> in float32 against differences of the 64-bit forward pass."""
     heads, dim, tokens = (3, 2, 1), 128, 6
