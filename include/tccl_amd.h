@@ -465,8 +465,8 @@ int tccl_qk_norm_rope_backward(const void *const *bufs, int world, const void *d
 /* A paged key/value cache in W buffers of tccl_paged_cache_bytes() each.  Pages are numbered over all ranks:
  * rank r holds pages [r * pages_per_rank, (r + 1) * pages_per_rank).  A slot is page * page_size + place in the
  * page.  dtype TCCL_E4M3 keeps every token's head as e4m3 codes times 2^e, e the least exponent >= -110
- * with 448 * 2^e >= the largest finite magnitude; infinities are kept as NaN.  The layout inside a page is the
- * library's own. */
+ * with 448 * 2^e >= the largest finite magnitude (for e = 120 the codes stop at 240, so that finite values stay
+ * finite); infinities are kept as NaN.  The layout inside a page is the library's own. */
 typedef struct {
     void *bufs[TCCL_MAX_WORLD];
     int world;

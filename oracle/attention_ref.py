@@ -56,7 +56,8 @@ def stored(x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
         e = torch.where((448.0 * 2.0 ** (n - 1) < largest) & (n > -110), float(n), e)
     y = x / torch.exp2(e)
     step = torch.exp2(torch.clamp(torch.floor(torch.log2(y.abs().clamp(min=2.0 ** -20, max=448.0))), min=-6.0) - 3)
-    y = torch.round(y / step) * step * torch.exp2(e)
+    y = torch.round(y / step) * step
+    y = torch.where(e == 120, y.clamp(-240.0, 240.0), y) * torch.exp2(e)     # 256 times 2^120 would be no finite number
     return torch.where(finite, y, math.nan)
 
 

@@ -104,7 +104,12 @@ __device__ __forceinline__ void turn_group(const uint32_t (&in)[16], uint32_t (&
     }
 }
 
-// A row with infinities or NaN: its scale comes from the largest finite magnitude, what is not finite becomes NaN.
+// Rows from here on take the path below: the fp32 bits of 1.9375 * 2^127, whose scale is 2^120 and whose code would round
+// to 256, that is 2^128.
+constexpr uint32_t kSpecialMagnitude = 0x7F780000u;
+
+// A row with infinities, NaN or the largest finite numbers: its scale comes from the largest finite magnitude, what is not
+// finite becomes NaN, and the codes of the largest scale stop at 240, so that no finite number becomes infinite.
 template <class Row, int LANES>
 __device__ __forceinline__ u32x2 codes_of_special_row(Row x, uint32_t &scale)
 {
@@ -119,10 +124,15 @@ __device__ __forceinline__ u32x2 codes_of_special_row(Row x, uint32_t &scale)
             largest = largest > u ? largest : u;
     }
     scale = scale_byte(f32_to_bits(reduce_row<MaxOp, LANES>(bits_to_f32(largest))));
-    u32x2 r = x.codes(scale_of(scale));
+    const u32x2 code = x.codes(scale_of(scale));
+    u32x2 r = {0, 0};
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-        if (nan & (1u << k)) r[k >> 2] |= 0x7Fu << (8 * (k & 3));
+    for (int k = 0; k < 8; ++k) {
+        uint32_t c = (code[k >> 2] >> (8 * (k & 3))) & 0xFFu;
+        if (scale == kLargestScale && (c & 0x7Fu) > kCode240) c = (c & 0x80u) | kCode240;
+        if (nan & (1u << k)) c |= 0x7Fu;
+        r[k >> 2] |= c << (8 * (k & 3));
+    }
     return r;
 }
 
@@ -133,7 +143,7 @@ __device__ __forceinline__ void encode(const Row &x, char *to, uint32_t &scale)
     if constexpr (Store::kScaled) {
         const uint32_t m = x.magnitude();
         u32x2 code;
-        if (__any(m >= 0x7F800000u)) {
+        if (__any(m >= kSpecialMagnitude)) {
             code = codes_of_special_row<Row, LANES>(x, scale);
         } else {
             scale = scale_byte(f32_to_bits(reduce_row<MaxOp, LANES>(bits_to_f32(m))));

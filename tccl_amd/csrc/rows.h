@@ -200,7 +200,8 @@ constexpr int kLeastExponent = -110;
 // The exponent e of a row's scale 2^e, biased by 127, from the bits of its largest finite magnitude:
 // the least e with 448 * 2^e >= largest (448 = 1.75 * 2^8 is the largest e4m3 value).  A power of two makes
 // the division exact and every stored value a bf16 number; it costs no precision, since e4m3 is a
-// floating-point type itself.
+// floating-point type itself.  Of the largest scale, 2^120, only codes up to 240 are used: 256 * 2^120 is no finite number.
+constexpr uint32_t kLargestScale = 120 + 127, kCode240 = 0x77;
 __device__ __forceinline__ uint32_t scale_byte(uint32_t largest_bits)
 {
     const int e = static_cast<int>(largest_bits >> 23) - 127 - 8 + ((largest_bits & 0x7FFFFFu) > 0x600000u ? 1 : 0);

@@ -361,6 +361,34 @@ def test_cache_special_rows(store):
     assert torch.equal(bits(k), bits(v))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_cache_keeps_the_largest_finite_rows_finite_in_8_bits(dtype):
+    """Rows up to the type's largest number: the largest exponent's codes stop where a larger one would stand for 2^128."""
+    dim, top = 64, torch.finfo(dtype).max
+    largest = torch.tensor([1.75 * 2.0 ** 127, 1.78125 * 2.0 ** 127, 1.921875 * 2.0 ** 127, 1.9375 * 2.0 ** 127, -1.9375 * 2.0 ** 127,
+                            1.953125 * 2.0 ** 127, top, -top], dtype=torch.float64)
+    x = torch.randn(3 * len(largest), 1, dim, generator=torch.Generator().manual_seed(6)) * 1e37
+    x[:, 0, 5] = largest.repeat(3).float()
+    x[8:16, 0, 9], x[8:16, 0, 10] = math.nan, -math.inf       # beside what is not finite
+    x[16:, 0, 20:40] = largest[:, None].float() * torch.linspace(0.9, 1, 20)
+    x = x.to(dtype)
+    assert torch.isfinite(x[:8]).all() and torch.isfinite(x[16:]).all()
+    cache = tccl_amd.PagedCache(2, 2, 16, 1, dim, dtype=E4M3, device=DEV)
+    slots = torch.arange(len(x)) + 3
+    tccl_amd.cache_write(cache, x.to(DEV), x.flip(0).to(DEV), slots.to(DEV))
+    for as_dtype in (BF16, F32):
+        k, v = read_back(cache, slots, as_dtype)
+        assert_stored(k, x, E4M3, "k")
+        assert_stored(v, x.flip(0), E4M3, "v")
+        assert torch.isfinite(k[:8]).all() and torch.isfinite(k[16:]).all()
+    # a sequence of one token returns the token's values as they are kept
+    table, n = torch.tensor([[0]], dtype=torch.int32, device=DEV), torch.tensor([1], dtype=torch.int32, device=DEV)
+    for t in (0, 3, 6, 7):
+        tccl_amd.cache_write(cache, torch.zeros_like(x[:1]).to(DEV), x[t: t + 1].to(DEV), torch.tensor([0], device=DEV))
+        out = tccl_amd.decode_attention(torch.ones(1, 1, dim, dtype=BF16, device=DEV), cache, table, n)
+        assert torch.equal(out[0].cpu().double(), ref.stored(x[t], E4M3)), t
+
+
 def test_cache_takes_strided_sources():
     """k and v as views of one projection's rows, and a head-major tensor."""
     heads, dim, tokens = 3, 128, 50

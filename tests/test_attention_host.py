@@ -314,3 +314,12 @@ def test_reference_storage():
 def _exponent(y):
     m, e = torch.frexp(y.abs().amax(-1, keepdim=True))
     return e - 9 + (m > 0.875).int()
+
+
+def test_reference_storage_of_the_largest_rows():
+    """Multiples of 2^120 stop at 240: a finite value is kept as a finite one, off by at most half a step of a code, 2^-4 of it."""
+    x = torch.tensor([1.75, 1.9374, 1.9375, -1.9375, 2 - 2.0 ** -23], dtype=torch.float64)[:, None] * 2.0 ** 127
+    got = ref.stored(x, torch.float8_e4m3fn)
+    assert torch.equal(got[:, 0] / 2.0 ** 120, torch.tensor([224.0, 240.0, 240.0, -240.0, 240.0], dtype=torch.float64))
+    assert torch.isfinite(got.to(torch.bfloat16)).all() and torch.isfinite(got.float()).all()
+    assert ((got - x).abs() <= 2.0 ** -4 * x.abs()).all()
