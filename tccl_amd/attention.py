@@ -201,7 +201,11 @@ class PagedCache:
 
     ``dtype``: ``torch.bfloat16``, or ``torch.float8_e4m3fn`` with one power-of-two scale per token and head, formed as
     the token is written; stored values are bfloat16 numbers either way.  The layout inside a page is the library's own.
-    A new cache holds zeros."""
+    A new cache holds zeros.
+
+    Its buffers come from the current stream, which another stream has to wait for before it uses the cache.  It may be
+    dropped while streams still work on it: the allocator keeps the buffers until those that it was used on have passed
+    that point.  A captured graph holds their addresses only, so the cache has to live as long as the graph is replayed."""
 
     def __init__(self, world_size: int, pages_per_rank: int, page_size: int, kv_heads: int, head_dim: int, *,
                  dtype: torch.dtype = torch.bfloat16, device="cuda"):
@@ -227,6 +231,17 @@ class PagedCache:
             desc.bufs[r] = p
         self._desc = desc
         self._ref = ctypes.byref(desc)
+        self._streams = {_stream(self.device).value} if self.device.type == "cuda" else set()
+
+    def _launch_stream(self) -> ctypes.c_void_p:
+        """The current stream.  The first launch on one that the buffers do not come from tells the allocator of it."""
+        stream = _stream(self.device)
+        if stream.value not in self._streams and not torch.cuda.is_current_stream_capturing():    # (capturing runs nothing)
+            current = torch.cuda.current_stream(self.device)
+            for t in self.group.tensors:
+                t.record_stream(current)
+            self._streams.add(stream.value)
+        return stream
 
     def _rows(self, tokens: int) -> Tuple[int, int, int]:
         return tokens, self.kv_heads, self.head_dim
@@ -247,7 +262,7 @@ def cache_write(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, slots: torc
         return
     with _on(cache.device):
         rc = _lib.load().tccl_cache_write(cache._ref, k.data_ptr(), v.data_ptr(), *strides, slots.data_ptr(), tokens,
-                                          dtype, _stream(cache.device))
+                                          dtype, cache._launch_stream())
     _lib.check("tccl_cache_write", rc)
 
 
@@ -273,7 +288,7 @@ def cache_read(cache: PagedCache, slots: torch.Tensor, *, dtype: torch.dtype = t
             _aligned(v, "out[1]")
             with _on(cache.device):
                 rc = _lib.load().tccl_cache_read(cache._ref, slots.data_ptr(), tokens, k.data_ptr(), v.data_ptr(), code,
-                                                 _stream(cache.device))
+                                                 cache._launch_stream())
             _lib.check("tccl_cache_read", rc)
     return k, v
 
@@ -336,7 +351,7 @@ def decode_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tenso
                 rc = _lib.load().tccl_decode_attention(
                     cache._ref, q.data_ptr(), *q_strides, page_table.data_ptr(), row, lengths.data_ptr(), out.data_ptr(),
                     lse.data_ptr() if lse is not None else None, workspace.data_ptr() if nbytes else None, nbytes, batch, q_heads,
-                    most, scale, _stream(device))
+                    most, scale, cache._launch_stream())
             _lib.check("tccl_decode_attention", rc)
     return (out, lse) if lse is not None else out
 

@@ -735,6 +735,36 @@ def test_on_another_stream_and_two_at_once():
         check_attention(out, lse, q, keys, values)
 
 
+@pytest.mark.parametrize("call", ["write", "read", "attention"])
+def test_a_cache_dropped_while_another_stream_uses_it(call):
+    """The buffers are not handed out again before that stream has passed the call."""
+    cache, table, n, q, keys, values, slots = filled(2, [700, 100], 8, 2, 128, 16, BF16, seed=1)
+    at, queries = torch.cat(slots).to(DEV), q.to(DEV)
+    k, v = (torch.cat(x).to(BF16).to(DEV) for x in (keys, values))
+    nbytes, pointers = cache.group.tensors[0].numel(), set(cache.group.buffer_ptrs)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)
+        if call == "write":
+            tccl_amd.cache_write(cache, k, v, at)
+        elif call == "read":
+            got = tccl_amd.cache_read(cache, at)
+        else:
+            out = tccl_amd.decode_attention(queries, cache, table, n)
+    del cache
+    others = [torch.full((nbytes,), 0xFF, dtype=torch.uint8, device=DEV) for _ in range(2)]
+    assert not side.query(), "the side stream was to be busy still"
+    assert pointers.isdisjoint(t.data_ptr() for t in others)
+    torch.cuda.synchronize()
+    if call == "write":
+        assert all((t == 0xFF).all() for t in others)
+    elif call == "read":
+        assert torch.equal(got[0], k) and torch.equal(got[1], v)
+    else:
+        check_attention(out, None, q, keys, values)
+
+
 def captured(fn):
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())

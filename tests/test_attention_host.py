@@ -13,7 +13,7 @@ import torch
 
 import tccl_amd
 from oracle import attention_ref as ref
-from tccl_amd import _lib
+from tccl_amd import _lib, attention
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 OK, EINVAL, EALIGN, ESCRATCH = _lib.TCCL_OK, _lib.TCCL_EINVAL, _lib.TCCL_EALIGN, _lib.TCCL_ESCRATCH
@@ -231,6 +231,35 @@ def test_paged_cache_refusals():
         tccl_amd.cache_read(cache, slots, dtype=torch.float32, out=(torch.zeros(641)[1:].view(5, 2, 64), k))
     with pytest.raises(ValueError, match="GPU"):
         tccl_amd.cache_read(cache, slots)
+
+
+def test_a_cache_tells_the_allocator_of_other_streams_once(monkeypatch):
+    """So that a dropped cache's buffers stay its own until work on those streams is done."""
+    cache = tccl_amd.PagedCache(2, 3, 16, 2, 64, device="cpu")
+    told = []
+
+    class Buffer:
+        def record_stream(self, stream):
+            told.append((self, stream))
+
+    buffers = cache.group.tensors = [Buffer(), Buffer()]
+    cache._streams = {None}                                            # made on the default stream
+    state = {"raw": None, "capturing": False}
+    monkeypatch.setattr(attention, "_stream", lambda device: ctypes.c_void_p(state["raw"]))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: state["capturing"])
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device: f"stream {state['raw']}")
+
+    def launch(raw, capturing=False):
+        state.update(raw=raw, capturing=capturing)
+        del told[:]
+        assert cache._launch_stream().value == raw
+        return told
+
+    assert launch(None) == []
+    assert launch(7, capturing=True) == []                             # nothing runs
+    assert launch(7) == [(buffers[0], "stream 7"), (buffers[1], "stream 7")]
+    assert launch(7) == [] and launch(None) == []
+    assert len(launch(8)) == 2 and launch(7) == []
 
 
 def test_decode_attention_refusals():
