@@ -223,6 +223,7 @@ class PagedCache:
         desc.world, desc.pages_per_rank, desc.page_size = world_size, pages_per_rank, page_size
         desc.kv_heads, desc.head_dim, desc.dtype = kv_heads, head_dim, _STORES[dtype]
         nbytes = _lib.load().tccl_paged_cache_bytes(ctypes.byref(desc))
+        _need(nbytes > 0, "a rank's buffer must be under 2^63 bytes")
         # a group of its own, but not one that rendezvous finds: its buffers are no operand of a collective
         self.group = SymmGroup([torch.zeros(nbytes, dtype=torch.uint8, device=device) for _ in range(world_size)])
         self.group.handles.clear()     # (they point back at the group: the buffers would outlive the cache until a collection)

@@ -366,7 +366,9 @@ static int check_geometry(const tccl_paged_cache *c)
     if (c->page_size < 16 || c->page_size > 256 || (c->page_size & (c->page_size - 1)) != 0) return TCCL_EINVAL;
     if (c->kv_heads < 1 || c->kv_heads > 65535) return TCCL_EINVAL;
     if (c->pages_per_rank < 1 || static_cast<int64_t>(c->pages_per_rank) * c->world > 0x7FFFFFFF) return TCCL_EINVAL;
-    return TCCL_OK;
+    // below 2^47 blocks, of up to 2^18 bytes: a buffer's size has to fit its type
+    const size_t blocks = static_cast<size_t>(c->pages_per_rank) * c->kv_heads;
+    return blocks <= static_cast<size_t>(PTRDIFF_MAX) / block_bytes_of(*c) ? TCCL_OK : TCCL_EINVAL;
 }
 
 int check_cache(const tccl_paged_cache *c, PoolShape *shape)

@@ -233,6 +233,22 @@ def test_paged_cache_refusals():
         tccl_amd.cache_read(cache, slots)
 
 
+def test_a_cache_larger_than_an_address_space_is_refused():
+    """40,000 heads of 256 x 2 x 256 bf16: 2^64 bytes and 5.9 GB more, of which 64 bits would hold the 5.9 GB."""
+    lib = tccl_amd.load_library()
+    pages, heads = -(-(1 << 46) // 40_000), 40_000
+    assert pages * heads << 18 > 1 << 64 and pages < 1 << 31
+    big = dict(pages_per_rank=pages, kv_heads=heads, page_size=256, head_dim=256, world=1)
+    assert lib.tccl_paged_cache_bytes(desc(**big)) == 0
+    assert lib.tccl_cache_write(desc(**big), 0x1000, 0x2000, 256, 256, 256, 256, 0x3000, 0, 0, None) == EINVAL
+    assert lib.tccl_cache_read(desc(**big), 0x3000, 0, 0x1000, 0x2000, 0, None) == EINVAL
+    assert lib.tccl_decode_attention(desc(**big), 0x1000, 512, 256, 0x2000, 4, 0x3000, 0x4000, None, None, 0, 0, heads, 64, 0.1, None) == EINVAL
+    with pytest.raises(ValueError, match="bytes"):
+        tccl_amd.PagedCache(1, pages, 256, heads, 256, device="cpu")
+    half = dict(big, pages_per_rank=pages // 2 - 1)
+    assert lib.tccl_paged_cache_bytes(desc(**half)) == half["pages_per_rank"] * heads << 18
+
+
 def test_a_cache_tells_the_allocator_of_other_streams_once(monkeypatch):
     """So that a dropped cache's buffers stay its own until work on those streams is done."""
     cache = tccl_amd.PagedCache(2, 3, 16, 2, 64, device="cpu")
