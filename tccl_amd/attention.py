@@ -381,6 +381,7 @@ def attention_all_reduce(tensor: torch.Tensor, lse: torch.Tensor, *, out: Option
         if symm.world_size != symm_lse.world_size or symm.rank != symm_lse.rank:
             raise ValueError("attention_all_reduce: tensor and lse must be the same rank's buffers of two groups of one world")
         symm.group.check_signals()
+        symm_lse.group.check_signals()
         output = torch.empty_like(tensor) if out is None else _check_out(out, tensor.shape, tensor)
         output_lse = torch.empty_like(lse)
         _aligned(output, "out")

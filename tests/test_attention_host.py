@@ -313,6 +313,19 @@ def test_attention_all_reduce_refusals():
         tccl_amd.attention_all_reduce(o, l)
 
 
+@pytest.mark.parametrize("which", [0, 1])
+def test_attention_all_reduce_looks_at_both_groups_expired_waits(which, monkeypatch):
+    """Outputs or softmax sums that a collective left half reduced are not joined unnoticed."""
+    groups = [tccl_amd.empty_world(2, (6, 64), torch.float32, "cpu"), tccl_amd.empty_world(2, (6,), torch.float32, "cpu")]
+
+    def expired():
+        raise _lib.TcclError("a signalling collective", _lib.TCCL_ETIMEOUT, "a wait expired")
+
+    monkeypatch.setattr(groups[which], "check_signals", expired)
+    with pytest.raises(_lib.TcclError, match="wait expired"):
+        tccl_amd.attention_all_reduce(groups[0].tensor(0), groups[1].tensor(0))
+
+
 def test_groups_of_other_processes_are_refused():
     """The kernels read every rank's buffer without the in-kernel barrier that ranks in processes of their own need."""
     own = torch.zeros(4, 8 * 64, dtype=torch.bfloat16)
