@@ -87,6 +87,15 @@ def _heads_first(t: torch.Tensor, name: str) -> Tuple[int, int]:
     return token, head
 
 
+def _refuse_overlap(out: torch.Tensor, buffers: Tuple[int, ...], nbytes: int, in_place: bool) -> None:
+    """``out`` must not lie over the first ``nbytes`` of the ranks' buffers, except from one's very start if ``in_place``."""
+    start = out.data_ptr()
+    stop = start + out.numel() * out.element_size()
+    for p in buffers:
+        if start < p + nbytes and p < stop and not (in_place and start == p):
+            raise ValueError("out must not overlap what the ranks' launches read")
+
+
 # ---------------------------------------------------------------- sum, per-head norm and rotation
 
 def _norm_arguments(tensor, q_weight, k_weight, positions, inv_freq, heads, what):
@@ -311,7 +320,9 @@ def decode_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tenso
 
     Returns ``[batch, q_heads, head_dim]`` bfloat16 and, with ``return_lse`` or ``lse``, the logarithm of the softmax's
     sum, float32 ``[batch, q_heads]``: what ``attention_all_reduce`` joins parts with.  A sequence without tokens gives
-    0 and -inf.  Scores, softmax and sums are fp32; an infinite cached value gives NaN."""
+    0 and -inf.  Scores, softmax and sums are fp32; an infinite cached value gives NaN, and so may finite ones whose sum,
+    weighted by up to 1 each, passes fp32's range before it is divided.  ``out`` may be q itself where q is contiguous;
+    otherwise outputs must not overlap inputs."""
     batch, dim, device = lengths.numel(), cache.head_dim, cache.device
     if q.dtype != torch.bfloat16 or q.dim() != 3 or q.shape[0] != batch or q.shape[2] != dim or q.device != device:
         raise ValueError(f"q must be a bfloat16 tensor of shape [{batch}, q_heads, {dim}] on {device}")
@@ -365,7 +376,9 @@ def attention_all_reduce(tensor: torch.Tensor, lse: torch.Tensor, *, out: Option
     ``tensor``: this rank's ``[..., head_dim]`` buffer (bfloat16 or float32, head_dim 64, 128 or 256) of one symmetric
     group, ``lse``: its float32 ``[...]`` buffer of another, both as ``decode_attention(out=, lse=)`` fills them.  Returns
     the joined output and its lse, the same on every rank.  A rank whose lse is -inf is left out, whatever its buffer
-    holds; where all are, the output is 0 and lse -inf."""
+    holds; where all are, the output is 0 and lse -inf.  ``out`` may be a rank's buffer where this call is the only one (not
+    inside ``spmd.run``, where other ranks' launches still read it); any other overlap is refused.  The weighted sum is fp32
+    and divided at the end: finite values past 2^128 / world_size may give infinity."""
     dtype = _sum_dtype(tensor)
     if tensor.dim() < 1 or tensor.shape[-1] not in HEAD_DIMS:
         raise ValueError(f"attention_all_reduce: head_dim must be one of {HEAD_DIMS}")
@@ -383,6 +396,10 @@ def attention_all_reduce(tensor: torch.Tensor, lse: torch.Tensor, *, out: Option
         symm.group.check_signals()
         symm_lse.group.check_signals()
         output = torch.empty_like(tensor) if out is None else _check_out(out, tensor.shape, tensor)
+        if out is not None:
+            _refuse_overlap(out, symm.buffer_ptrs, lse.numel() * tensor.shape[-1] * tensor.element_size(),
+                            in_place=spmd.current_rank() is None or symm.world_size == 1)
+            _refuse_overlap(out, symm_lse.buffer_ptrs, lse.numel() * 4, in_place=False)
         output_lse = torch.empty_like(lse)
         _aligned(output, "out")
         with _on(tensor.device):

@@ -676,6 +676,26 @@ def test_attention_all_reduce(world, shape, dtype):
     assert_bit_equal(again, got, "another rank's call")
 
 
+def test_outputs_in_the_place_of_inputs():
+    """attention_all_reduce into one of the ranks' buffers and decode_attention into its queries: the same bits as apart."""
+    rng = torch.Generator().manual_seed(3)
+    outs, lses = [torch.randn(5000, 64, generator=rng) for _ in range(3)], [torch.randn(5000, generator=rng) for _ in range(3)]
+    o, l = world_of(outs), world_of(lses)
+    want, want_lse = tccl_amd.attention_all_reduce(o.tensor(0), l.tensor(0))
+    got, lse = tccl_amd.attention_all_reduce(o.tensor(0), l.tensor(0), out=o.tensor(1))
+    assert got is o.tensor(1)
+    assert_bit_equal(got, want, "in place")
+    assert_bit_equal(lse, want_lse, "in place, lse")
+    for lengths, heads in (([700, 3, 20011, 0], (6, 2)), ([40, 17], (70, 1))):            # split and not
+        cache, table, n, q, *_ = filled(2, lengths, *heads, 64, 16, BF16, seed=4)
+        queries = q.to(DEV)
+        want, want_lse = tccl_amd.decode_attention(queries, cache, table, n, return_lse=True)
+        got, lse = tccl_amd.decode_attention(queries, cache, table, n, out=queries, return_lse=True)
+        assert got is queries
+        assert_bit_equal(got, want, "in place of the queries")
+        assert_bit_equal(lse, want_lse, "lse")
+
+
 # ---------------------------------------------------------------- together, streams, graphs, per-rank programs
 
 @pytest.mark.parametrize("store", [BF16, E4M3])

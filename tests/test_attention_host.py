@@ -326,6 +326,31 @@ def test_attention_all_reduce_looks_at_both_groups_expired_waits(which, monkeypa
         tccl_amd.attention_all_reduce(groups[0].tensor(0), groups[1].tensor(0))
 
 
+def test_attention_all_reduce_refuses_outputs_that_other_reads_would_meet():
+    """A launch reads every rank's rows: an output over them is right row by row only, and not where each rank launches its own."""
+    outs, lses = tccl_amd.empty_world(2, (8, 64), torch.float32, "cpu"), tccl_amd.empty_world(2, (8,), torch.float32, "cpu")
+    o, l = outs.tensor(0)[:4], lses.tensor(0)[:4]
+    for out in (outs.tensor(0)[1:5], outs.tensor(1)[3:7]):
+        with pytest.raises(ValueError, match="overlap"):
+            tccl_amd.attention_all_reduce(o, l, out=out)
+    for out in (o, outs.tensor(1)[:4], outs.tensor(0)[4:], torch.zeros(4, 64)):     # in place, or apart: only the GPU is missing
+        with pytest.raises(ValueError, match="GPU"):
+            tccl_amd.attention_all_reduce(o, l, out=out)
+    few, sums = tccl_amd.empty_world(2, (1, 64), torch.float32, "cpu"), tccl_amd.empty_world(2, (256,), torch.float32, "cpu")
+    with pytest.raises(ValueError, match="overlap"):
+        tccl_amd.attention_all_reduce(few.tensor(0), sums.tensor(0)[:1], out=sums.tensor(1)[:64].view(1, 64))
+
+    def main(rank, world_size, peer):
+        t = tccl_amd.spmd.empty_strided_p2p((8, 64), None, torch.float32, "cpu")
+        s = tccl_amd.spmd.empty_strided_p2p((8,), None, torch.float32, "cpu")
+        tccl_amd.attention_all_reduce(t, s, out=t if peer is None else outs.tensor(0))
+
+    with pytest.raises(ValueError, match="overlap"):
+        tccl_amd.spmd.run(2, main, None)
+    with pytest.raises(ValueError, match="GPU"):
+        tccl_amd.spmd.run(2, main, 1)
+
+
 def test_groups_of_other_processes_are_refused():
     """The kernels read every rank's buffer without the in-kernel barrier that ranks in processes of their own need."""
     own = torch.zeros(4, 8 * 64, dtype=torch.bfloat16)
