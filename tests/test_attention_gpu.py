@@ -205,6 +205,36 @@ def test_qk_norm_rope_any_eps_with_heads_and_tokens_missing(case, eps):
     check_backward(got, parts, w, positions, inv_freq, grads, heads, eps, interleaved, sum(heads))
 
 
+ROUND_CASES = [
+    # world, tokens, heads, dim, rotary, interleaved, dtype, tokens per workgroup (a wave's share of heads: 512 elements)
+    (1, 4099, (16, 8, 8), 64, 64, False, BF16, 1),
+    (1, 2600, (10, 5, 0), 128, 32, True, F32, 1),
+    (8, 2600, (12, 6, 7), 64, 64, True, F32, 1),
+    (2, 4003, (4, 2, 1), 128, 128, False, BF16, 2),
+    (2, 13_003, (3, 1, 1), 64, 16, False, F32, 4),
+]
+
+
+@pytest.mark.parametrize("case", ROUND_CASES, ids=lambda c: "-".join(str(x).replace("torch.", "") for x in c))
+def test_qk_norm_rope_backward_over_several_rounds_of_tokens(case):
+    """More tokens than the workgroups that run at once (five per compute unit at most) take: each walks on with the grid's stride,
+    writes other angles into the same LDS and keeps its sums."""
+    world, tokens, heads, dim, rotary, interleaved, dtype, at_once = case
+    workgroups = -(-tokens // at_once)
+    least = torch.cuda.get_device_properties(0).multi_processor_count * 3          # of the eight-source fp32 kernel
+    most = least // 3 * (3 if world > 6 else 4 if dtype == F32 else 5)
+    assert workgroups > most
+    parts, w, positions, inv_freq, grads = norm_inputs(world, tokens, heads, dim, rotary, dtype, seed=tokens)
+    group = world_of(parts)
+    dev = [t.to(DEV) for t in (*w, positions, inv_freq)]
+    got = tccl_amd.qk_norm_rope_backward(*(g.to(DEV) for g in grads), group.tensor(0), *dev, interleaved=interleaved)
+    rounds = -(-workgroups // least)
+    check_backward(got, parts, w, positions, inv_freq, grads, heads, 1e-6, interleaved, sum(heads) * at_once * rounds)
+    again = tccl_amd.qk_norm_rope_backward(*(g.to(DEV) for g in grads), group.tensor(0), *dev, interleaved=interleaved)
+    for a, b in zip(got, again):
+        assert_bit_equal(a, b, "the same call twice")
+
+
 def test_qk_norm_rope_backward_against_differences():
     """<dx, d> and <dw, d> in float32 against differences of the 64-bit forward pass."""
     heads, dim, tokens = (3, 2, 1), 128, 6
