@@ -562,6 +562,31 @@ def test_decode_attention(case):
     check_attention(out, lse, q, keys, values, what="max_length")
 
 
+WIDE_CASES = [
+    # more than 64 query heads on one key head: several workgroups per sequence and key head
+    (2, [300, 0, 40], 65, 1, 64, 16, BF16),
+    (1, [130, 17], 200, 2, 128, 32, E4M3),
+    (3, [90, 1], 100, 1, 256, 64, E4M3),
+    (1, [5003, 0, 700], 128, 1, 128, 64, E4M3),
+    (4, [3001, 1, 900], 100, 1, 256, 16, BF16),
+    (2, [9000, 20], 260, 2, 64, 32, BF16),
+    # either side of where a fourth wave begins to help: two and three blocks of 16
+    (2, [1500, 33], 32, 1, 128, 16, BF16),
+    (2, [1500, 33], 33, 1, 128, 16, E4M3),
+    (2, [1500, 33], 64, 1, 64, 16, E4M3),
+]
+
+
+@pytest.mark.parametrize("case", WIDE_CASES, ids=lambda c: f"w{c[0]}-n{len(c[1])}x{max(c[1])}-q{c[2]}-k{c[3]}-d{c[4]}-p{c[5]}-{str(c[6])[6:]}")
+def test_decode_attention_many_query_heads_on_a_key_head(case):
+    cache, table, n, q, keys, values, _ = filled(*case, seed=8)
+    out, lse = tccl_amd.decode_attention(q.to(DEV), cache, table, n, return_lse=True)
+    check_attention(out, lse, q, keys, values)
+    again, lse_again = tccl_amd.decode_attention(q.to(DEV), cache, table, n, return_lse=True)
+    assert_bit_equal(out, again, "twice")
+    assert_bit_equal(lse, lse_again, "lse twice")
+
+
 @pytest.mark.parametrize("store", [BF16, E4M3])
 def test_decode_attention_peaked_scores_and_scales(store):
     """Scores far apart (a weight underflows to zero), far below zero, and a caller's scale."""
