@@ -588,6 +588,37 @@ def test_decode_attention_many_query_heads_on_a_key_head(case):
 
 
 @pytest.mark.parametrize("store", [BF16, E4M3])
+def test_decode_attention_more_pages_than_a_workgroup_looks_up_at_once(store):
+    """A workgroup looks 512 page addresses up at a time.  Here each one's even share is over 8,192 tokens of 16 per page, so that it
+    looks up again, in the middle of a sequence and after it has gone on to the next; peaked scores make every part count."""
+    world, kv_heads, group, dim, page = 2, 8, 2, 64, 16
+    shares = 2 * torch.cuda.get_device_properties(0).multi_processor_count
+    lengths = [83_001, 0, 79_990, 8_193, 80_000, 1, 77_777, 90_111, 85_003, 81_920, 64_005]
+    assert sum(lengths) * kv_heads / shares > 1.2 * 512 * page
+    rng = torch.Generator(device=DEV).manual_seed(9)
+    used = [-(-n // page) for n in lengths]
+    cache = tccl_amd.PagedCache(world, -(-sum(used) // world), page, kv_heads, dim, dtype=store, device=DEV)
+    ids = torch.randperm(cache.pages, generator=rng, device=DEV)[: sum(used)].split(used)
+    table = torch.full((len(lengths), max(used)), -1, dtype=torch.int32, device=DEV)
+    keys, values = [], []
+    for b, n in enumerate(lengths):
+        table[b, : used[b]] = ids[b].int()
+        t = torch.arange(n, device=DEV)
+        k, v = (torch.randn(n, kv_heads, dim, generator=rng, device=DEV).to(BF16) for _ in range(2))
+        if n:
+            tccl_amd.cache_write(cache, k, v, ids[b][t // page] * page + t % page)
+        keys.append(k)
+        values.append(v)
+    q = torch.randn(len(lengths), kv_heads * group, dim, generator=rng, device=DEV).to(BF16)
+    out, lse = tccl_amd.decode_attention(q, cache, table, torch.tensor(lengths, dtype=torch.int32, device=DEV), scale=0.6, return_lse=True)
+    for b in range(len(lengths)):
+        for h in range(b % 3, kv_heads, 3):
+            heads = slice(h * group, (h + 1) * group)
+            kept = [ref.stored(x[b][:, h: h + 1].cpu(), store) for x in (keys, values)]
+            check_attention(out[b: b + 1, heads], lse[b: b + 1, heads], q[b: b + 1, heads].cpu(), [kept[0]], [kept[1]], 0.6, f"{b} {h}")
+
+
+@pytest.mark.parametrize("store", [BF16, E4M3])
 def test_decode_attention_peaked_scores_and_scales(store):
     """Scores far apart (a weight underflows to zero), far below zero, and a caller's scale."""
     cache, table, n, q, keys, values, _ = filled(2, [500, 77], 8, 2, 128, 32, store, seed=3, spread=8.0)
