@@ -459,6 +459,26 @@ def test_cache_behind_four_gib(store):
     check_attention(out, lse, q, [k.double()], [v.double()])
 
 
+@pytest.mark.parametrize("store", [BF16, E4M3])
+def test_cache_far_slots_and_given_outputs(store):
+    """Slots at both ends of int64 are padding; outputs that the caller gives are filled whole and nothing beside them."""
+    heads, dim = 2, 64
+    cache = tccl_amd.PagedCache(2, 3, 32, heads, dim, dtype=store, device=DEV)
+    x = torch.randn(6, heads, dim, generator=torch.Generator().manual_seed(14)).to(BF16)
+    slots = torch.tensor([-2 ** 63, 70, 2 ** 63 - 1, 71, cache.slots, 2 ** 40])
+    tccl_amd.cache_write(cache, x.to(DEV), x.to(DEV), slots.to(DEV))
+    for dtype in (BF16, F32):
+        wide = torch.full((3, 8, heads, dim), 9.0, dtype=dtype, device=DEV)
+        got = tccl_amd.cache_read(cache, slots.to(DEV), dtype=dtype, out=(wide[0, 1:7], wide[2, :6]))
+        assert got[0].data_ptr() == wide[0, 1].data_ptr() and got[1].data_ptr() == wide[2].data_ptr()
+        for t in got:
+            assert_stored(t.cpu()[1::2][:2], x[1::2][:2], store, "written")
+            assert not t[::2].any() and not t[5].any()
+        assert (wide[1] == 9).all() and (wide[0, 0] == 9).all() and (wide[0, 7] == 9).all() and (wide[2, 6:] == 9).all()
+    everything = tccl_amd.cache_read(cache, torch.arange(cache.slots, device=DEV))
+    assert sorted(torch.nonzero(everything[0].any(-1).any(-1))[:, 0].tolist()) == [70, 71]
+
+
 def test_cache_without_tokens():
     cache = tccl_amd.PagedCache(1, 1, 16, 2, 64, device=DEV)
     none = torch.empty(0, 2, 64, device=DEV)
@@ -731,6 +751,27 @@ def test_decode_attention_nan_in_a_live_token_reaches_its_heads_only():
     assert bad[0, :2].all() and bad.sum() == 2 * 64
 
 
+@pytest.mark.parametrize("store", [BF16, E4M3])
+def test_decode_attention_of_sequences_that_share_pages(store):
+    """A prefix in the cache once for all sequences, as a table row for all (a stride of 0) and as rows that part later; a length of
+    2^31 - 1 is what the table has room for."""
+    cache, table, n, q, keys, values, _ = filled(2, [700, 64, 130], 8, 2, 64, 16, store, seed=12)
+    one = table[:1, :44].expand(3, 44)
+    lengths = [700, 33, 2 ** 31 - 1]
+    out, lse = tccl_amd.decode_attention(q.to(DEV), cache, one, torch.tensor(lengths, dtype=torch.int32, device=DEV), return_lse=True)
+    have = [700, 33, 704]
+    written = [torch.cat((x[0], torch.full((4, 2, 64), math.nan).double())) for x in (keys, values)]       # 4 tokens nobody wrote
+    check_attention(out[:2], lse[:2], q[:2], [written[0][:m] for m in have[:2]], [written[1][:m] for m in have[:2]])
+    assert torch.isnan(out[2]).all() and torch.isnan(lse[2]).all()
+    mixed = table[:, :44].clone()
+    mixed[1:, :4] = table[0, :4]
+    mixed[2, 4:9] = table[2, :5]
+    n = torch.tensor([700, 64, 64 + 80], dtype=torch.int32, device=DEV)
+    out, lse = tccl_amd.decode_attention(q.to(DEV), cache, mixed, n, return_lse=True)
+    held = [[x[0], x[0][:64], torch.cat((x[0][:64], x[2][:80]))] for x in (keys, values)]
+    check_attention(out, lse, q, *held)
+
+
 # ---------------------------------------------------------------- the join over ranks
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
@@ -915,6 +956,40 @@ def test_a_decode_step_in_two_graphs():
             kept = [t.clone() for t in result]
             for got, want in zip(kept, step()):
                 assert_bit_equal(got, want, f"replay {turn}")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_parts_and_their_join_in_a_graph(dtype):
+    """Each rank's attention over its own pages into symmetric buffers and their join, captured and replayed over new queries."""
+    world, lengths = 3, [900, 40, 0]
+    parts = [filled(1, lengths, 8, 2, 64, 16, BF16, seed=20 + r) for r in range(world)]
+    q = parts[0][3].to(DEV)
+    outs = tccl_amd.empty_world(world, (3, 8, 64), BF16, DEV)
+    lses = tccl_amd.empty_world(world, (3, 8), F32, DEV)
+    wide = tccl_amd.empty_world(world, (3, 8, 64), dtype, DEV)
+
+    def step():
+        for r, (cache, table, n, *_) in enumerate(parts):
+            tccl_amd.decode_attention(q, cache, table, n, out=outs.tensor(r), lse=lses.tensor(r))
+            wide.tensor(r).copy_(outs.tensor(r))
+        return tccl_amd.attention_all_reduce(wide.tensor(1), lses.tensor(1))
+
+    graph, result = captured(step)
+    rng = torch.Generator(device=DEV).manual_seed(1)
+    for turn in range(4):
+        q.copy_(torch.randn(q.shape, generator=rng, device=DEV))
+        graph.replay()
+        torch.cuda.synchronize()
+        kept = [t.clone() for t in result]
+        for got, want in zip(kept, step()):
+            assert_bit_equal(got, want, f"replay {turn}")
+        keys = [torch.cat([p[4][b] for p in parts]) for b in range(3)]
+        values = [torch.cat([p[5][b] for p in parts]) for b in range(3)]
+        want, want_lse = ref.attention(q.cpu(), keys, values)
+        magnitude, _ = ref.attention(q.cpu(), keys, [v.abs() for v in values])
+        # as in test_a_serving_step_over_ranks: the parts' rounding to bf16, the joint's, and what the parts are off by
+        within(kept[0], want, 2 * half_step(BF16) * magnitude * (1 + 2.0 ** -6) + 2.0 ** -12 * magnitude, "joined")
+        within(kept[1], want_lse, 2.0 ** -14 * (1 + torch.nan_to_num(want_lse.abs(), posinf=0.0)), "joined lse")
 
 
 def test_in_a_per_rank_program():
