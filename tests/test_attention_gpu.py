@@ -301,6 +301,29 @@ def test_norm_without_tokens_and_with_a_prefix_view():
     check_forward(got, [p[:5] for p in parts], w, positions[:5], inv_freq, (2, 1, 1), 1e-6, False)
 
 
+def test_norm_of_buffers_behind_four_gib():
+    """Offsets that pass 32 bits, in elements and in bytes: only the last tokens are other than zero, and carry gradients."""
+    heads, dim, some = (20, 4, 4), 128, 5
+    columns = sum(heads) * dim
+    tokens = (9 << 30) // (2 * columns) | 1                              # 4.8e9 elements
+    last, w, _, inv_freq, grads = norm_inputs(1, some, heads, dim, dim, BF16, seed=17)
+    positions = torch.arange(tokens)
+    x = torch.zeros(tokens, columns, dtype=BF16, device=DEV)
+    x[-some:] = last[0].to(DEV)
+    group = tccl_amd.register([x])
+    dev = [t.to(DEV) for t in (*w, positions, inv_freq)]
+    got = tccl_amd.qk_norm_rope(x, *dev, heads[0], heads[1])
+    check_forward([t[-some:] for t in got], last, w, positions[-some:], inv_freq, heads, 1e-6, False)
+    assert not any(t[:1000].any() or t[-some - 1000:-some].any() for t in got)
+    for t, g in zip(got, grads):
+        t.zero_()
+        t[-some:] = g.to(DEV)
+    dx, *dw = tccl_amd.qk_norm_rope_backward(*got, x, *dev)
+    check_backward([dx[-some:], *dw], last, w, positions[-some:], inv_freq, grads, heads, 1e-6, False, some * sum(heads))
+    assert not dx[:1000].any() and not dx[-some - 1000:-some].any()
+    tccl_amd.unregister(group)
+
+
 # ---------------------------------------------------------------- the paged cache
 
 def read_back(cache, slots, dtype=BF16):
@@ -801,6 +824,24 @@ def test_attention_all_reduce(world, shape, dtype):
     again, _ = tccl_amd.attention_all_reduce(o.tensor(0), l.tensor(0), out=into)
     assert again is into
     assert_bit_equal(again, got, "another rank's call")
+
+
+def test_attention_all_reduce_behind_four_gib():
+    rows, dim, some = 36_000_007, 64, 9                                 # 2.3e9 elements, 4.6e9 bytes
+    rng = torch.Generator().manual_seed(18)
+    o, l = tccl_amd.empty_world(2, (rows, dim), BF16, DEV), tccl_amd.empty_world(2, (rows,), F32, DEV)
+    outs, lses = [torch.randn(some, dim, generator=rng).to(BF16) for _ in range(2)], [torch.randn(some, generator=rng) for _ in range(2)]
+    for r in range(2):
+        o.tensor(r).zero_()
+        l.tensor(r).fill_(-math.inf)
+        o.tensor(r)[-some:] = outs[r].to(DEV)
+        l.tensor(r)[-some:] = lses[r].to(DEV)
+    got, lse = tccl_amd.attention_all_reduce(o.tensor(0), l.tensor(0))
+    want, want_lse = ref.join(outs, lses)
+    magnitude, _ = ref.join([x.double().abs() for x in outs], lses)
+    within(got[-some:], want, half_step(BF16) * want.abs() * (1 + 2.0 ** -7) + 16 * U * magnitude, "out")
+    within(lse[-some:], want_lse, 14 * U + 4 * U * want_lse.abs(), "lse")
+    assert not got[:-some].any() and (lse[:-some] == -math.inf).all()
 
 
 def test_outputs_in_the_place_of_inputs():
