@@ -1063,3 +1063,31 @@ def test_in_a_per_rank_program():
             assert_bit_equal(a, b, "every rank has the same")
         # equal weights over equal parts: the parts themselves, up to the fp32 division by the number of ranks
         within(r[4], r[3].double(), half_step(BF16) * r[3].double().abs() * 1.01, "joined")
+
+
+def test_caches_of_the_ranks_own_in_a_per_rank_program():
+    """Each rank makes a cache for its part of the tokens, attends to it, and the parts are joined."""
+    world, lengths, page = 3, [70, 5, 0], 16
+    rng = torch.Generator().manual_seed(22)
+    q = torch.randn(3, 4, 64, generator=rng).to(BF16)
+    k, v = ([torch.randn(world, n, 2, 64, generator=rng).to(BF16) for n in lengths] for _ in range(2))
+    table = torch.arange(15, dtype=torch.int32).view(3, 5)
+
+    def main(rank, world_size):
+        cache = tccl_amd.PagedCache(1, 15, page, 2, 64, device=DEV)
+        slots = torch.cat([b * 5 * page + torch.arange(n) for b, n in enumerate(lengths)])
+        tccl_amd.cache_write(cache, *(torch.cat([t[rank] for t in x]).to(DEV) for x in (k, v)), slots.to(DEV))
+        out = tccl_amd.spmd.empty_strided_p2p((3, 4, 64), None, BF16, DEV)
+        lse = tccl_amd.spmd.empty_strided_p2p((3, 4), None, F32, DEV)
+        tccl_amd.decode_attention(q.to(DEV), cache, table.to(DEV), torch.tensor(lengths, dtype=torch.int32, device=DEV), out=out, lse=lse)
+        joined, joined_lse = tccl_amd.attention_all_reduce(out, lse)
+        return joined.cpu(), joined_lse.cpu()
+
+    results = tccl_amd.spmd.run(world, main)
+    keys, values = ([t.flatten(0, 1).double() for t in x] for x in (k, v))
+    want, want_lse = ref.attention(q, keys, values)
+    magnitude, _ = ref.attention(q, keys, [t.abs() for t in values])
+    for joined, joined_lse in results:
+        # as in test_a_serving_step_over_ranks
+        within(joined, want, 2 * half_step(BF16) * magnitude * (1 + 2.0 ** -6) + 2.0 ** -12 * magnitude, "joined")
+        within(joined_lse, want_lse, 2.0 ** -14 * (1 + torch.nan_to_num(want_lse.abs(), posinf=0.0)), "joined lse")
