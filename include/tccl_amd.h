@@ -442,7 +442,8 @@ int tccl_device_info(int *compute_units, int *mem_clock_khz, int *mem_bus_bits, 
  *
  * tccl_qk_norm_rope: one-shot all-reduce (sum) of `tokens` rows of q_heads + k_heads + v_heads heads whose epilogue
  * norms each query and key head (x / sqrt(mean x^2 + eps) * weight) and rotates its first rotary_dim elements
- * (a multiple of 16, at most head_dim) by the angles positions[t] * inv_freq[i], i < rotary_dim / 2.
+ * (a multiple of 16, at most head_dim) by the angles positions[t] * inv_freq[i], i < rotary_dim / 2.  eps >= 0; with
+ * eps = 0 a head of zeros gives NaN.
  * Pair i is elements (i, i + rotary_dim / 2), or (2i, 2i + 1) if `interleaved`.  The sum, norm and rotation are
  * fp32 and rounded once.  Outputs are [tokens][heads][head_dim] each; a kind with no heads may have a NULL output. */
 int tccl_qk_norm_rope(const void *const *bufs, int world, void *q_out, void *k_out, void *v_out,
@@ -488,7 +489,8 @@ int tccl_cache_write(const tccl_paged_cache *cache, const void *k, const void *v
                      const int64_t *slots, size_t tokens, int dtype, void *stream);
 
 /* Reads slots[t] into k_out and v_out [tokens][kv_heads][head_dim] (dtype bf16 or fp32: both hold the stored
- * values exactly).  A slot below 0 or outside the pool reads as zeros. */
+ * values exactly).  A slot below 0 or outside the pool reads as zeros.  Any order is right; tokens that follow each
+ * other cost least, since of every 8 (bf16) or 16 (8 bits) neighbouring tokens' values all are read for one. */
 int tccl_cache_read(const tccl_paged_cache *cache, const int64_t *slots, size_t tokens, void *k_out,
                     void *v_out, int dtype, void *stream);
 
@@ -508,7 +510,8 @@ int tccl_decode_attention(const tccl_paged_cache *cache, const void *q, size_t q
 
 /* Joins `world` partial attentions over disjoint tokens: out = sum_i w_i outs[i] / sum_i w_i with
  * w_i = exp(lses[i] - max), lse = max + log sum_i w_i; rows of head_dim elements (dtype bf16 or fp32), lses
- * fp32.  A source whose lse is -inf is not used; where all are, out is 0 and lse -inf. */
+ * fp32.  A source whose lse is -inf is not used; where all are, out is 0 and lse -inf.  out may be one of outs where
+ * no other launch reads them meanwhile; any other overlap is the caller's to avoid. */
 int tccl_attention_all_reduce(const void *const *outs, const void *const *lses, int world, void *out,
                               float *lse, size_t rows, int head_dim, int dtype, void *stream);
 

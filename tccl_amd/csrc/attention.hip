@@ -8,7 +8,7 @@
 // in any grouping.  No tokens give o = 0 and lse = -inf.
 //
 // The cache is read once; that is the floor, and HBM the bound: 64 sequences of 2,048 to 8,192 tokens of 8 key heads
-// of 128 in 8 bits take 115 us in the kernel, 5.9 TB/s (a large sum of torch reads at 6.2), with vector instructions a
+// of 128 in 8 bits take 117 us in the kernel, 5.8 TB/s (a large sum of torch reads at 6.2), with vector instructions a
 // third and matrix instructions a tenth of the time.  Scores come as S^T = K Q^T and the output as
 // O^T = V^T P^T from 16x16x32 matrix instructions: the cache's layout makes every 16-byte load an operand as it stands,
 // and a lane's scores are the tokens that the lane holds of P, so nothing passes through LDS and a query head's
@@ -511,7 +511,7 @@ struct JoinArgs {
 
 // out = sum_i w_i o_i / sum_i w_i, w_i = exp(lse_i - max lse): W reads and one write per element, a vector per lane
 // with every source's load in flight, read once and so marked as streaming; a row whose lse is -inf is not used,
-// whatever it holds.  Bound by HBM: four fp32 sources of 34 MB 30 us, 5.6 TB/s.
+// whatever it holds.  Bound by HBM: four fp32 sources of 34 MB 31 us, 5.5 TB/s.
 template <class Sum, int NSRC>
 __global__ void __launch_bounds__(256)
 attention_join_kernel(JoinArgs<NSRC> a)
@@ -597,12 +597,18 @@ struct AttnPlan {
 };
 
 // How many workgroups share the tokens: two per compute unit (one of head_dim 256, whose registers fill it), but
-// no more than there are units.  Measured with 64 sequences of 2,048 to 8,192 tokens in 8 bits, 8 key heads: one 132 us,
-// two 122, three 135; with 3 of 50,000 to 200,000 and one key head of 256: one 97, two 107.  A workgroup per row
-// and no second launch instead
-//   - where no sequence has over 512 tokens: 32 x 500 tokens, 8 key heads 15.4 us against 19.5;
+// no more than there are units.  Times here and below are whole calls in a graph, lengths from a quarter of the longest
+// to the longest.  64 sequences of up to 8,192 tokens, 8 key heads of 128, in 8 bits: one 128 us, two 119, three
+// 130 (in bf16 207 to 208 all of them); 3 of up to 200,003 and one key head of 256: one 92, two 102.  A workgroup per row
+// and no second launch instead (bf16, 8 key heads of 128)
+//   - where no sequence has over 512 tokens: 32 x 500 tokens 13.5 us against 17.0 (32 x 1,000, which are shared: 25.6 against
+//     21.3, so that the border could lie higher);
 //   - where the rows alone fill the GPU eight times and none is so long that the last one would be waited for:
-//     512 x 500 tokens 123 us against 163, 256 x 1,000 126 against 133, but 128 x 2,000 136 against 126.
+//     512 x 500 tokens 110 us against 130, 256 x 1,000 111 against 120; 128 x 2,000, whose rows do not, 113 against 115.
+// Three blocks of 16 query heads and more on a key head: four waves on the same tokens, which share their loads (of three blocks
+// the fourth wave loads along and multiplies zeros).  33 heads on one key head, 8 x 40,000 tokens: 37 us with four waves,
+// 38 with two and so two workgroups, 55 with one and three (128 dims), 61, 68 and 92 (256), 34, 33 and 36 (128 in 8 bits);
+// 64 heads 39, 39 and 65; 68, 72 and 120; 37, 36 and 43.  Short rows lose by it: 64 x 500 tokens 21, 15 and 13 us.
 static AttnPlan plan_attention(size_t batch, int q_heads, int kv_heads, int head_dim, int most)
 {
     AttnPlan p = {};
@@ -633,8 +639,8 @@ template <class Store, int D>
 static hipError_t launch_attention(const AttnArgs &a, hipStream_t stream)
 {
     const size_t grid = a.workgroups > 0 ? a.workgroups : static_cast<size_t>(a.batch) * a.head_groups;
-    // what one wave alone reads is marked as streaming (64 x 8,192 tokens in 8 bits 118 us against 132), what waves share is
-    // not (24 heads on one key head 105 us against 136)
+    // what one wave alone reads is marked as streaming (64 x up to 8,192 tokens of 8 key heads in 8 bits 120 us against 136), what
+    // waves share is not (3 x up to 200,003 tokens, 24 heads on one key head of 256, 91 us against 114)
     if (a.blocks_per_wg == 1)
         hipLaunchKernelGGL((decode_attention_kernel<Store, D, true>), dim3(static_cast<unsigned>(grid)),
                            dim3(kAttnBlock), 0, stream, a);
@@ -644,8 +650,8 @@ static hipError_t launch_attention(const AttnArgs &a, hipStream_t stream)
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.workgroups == 0) return e;
     const unsigned rows = static_cast<unsigned>(a.batch) * a.q_heads;
-    // four waves per row where a row has eight parts or more on average: 72 rows of 85 parts 8 us against 44, while
-    // 4,096 rows of two or three take 5 us with one against 8
+    // four waves per row where a row has eight parts or more on average: 72 rows of 85 parts 8 us against 28 with one, while
+    // 4,096 rows of two or three take 5 us with one against 11
     if (static_cast<size_t>(a.workgroups) >= 8 * static_cast<size_t>(a.batch) * a.head_groups)
         hipLaunchKernelGGL((join_parts_kernel<D, 4>), dim3(rows), dim3(256), 0, stream, a);
     else

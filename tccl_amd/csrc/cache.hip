@@ -11,8 +11,12 @@
 // ends inside) what is whole of each four bytes, the rest element by element, since its neighbours may be
 // written by another workgroup.
 //
-// Reading 44,000 tokens of 8 heads of 128 from 8 bits takes 56 us (4.8 TB/s, two thirds of it written), writing 8,192 of
-// them 18 us (2.8 TB/s: one wave of workgroups, whose reads, rounding and stores follow each other).
+// Tokens that do not follow each other are runs of one: each of them reads its whole group, 8 or 16 times its values.
+//
+// 8 heads of 128, bf16 rows, in the kernel.  Reading 44,000 tokens: from 8 bits 49 to 58 us from process to process (4.7 to
+// 5.6 TB/s, two thirds of it written), from bf16 73 us (5.0 TB/s).  Writing 8,192 of them that begin inside groups: in 8 bits 17.5 us
+// (2.9 TB/s), in bf16 21.0 (3.2): a single residency of workgroups, in each of which loads, rounding, turning and stores
+// follow each other; from a group's start 8,000 take 14.0 and 15.9 us where from inside one 17.9 and 19.2.
 #include "host.h"
 #include "rows.h"
 
@@ -398,8 +402,10 @@ static hipError_t launch_cache_tokens(bool write, const CacheArgs &a, hipStream_
     return hipGetLastError();
 }
 
-// Tiles of 64 tokens where they fill the GPU twice, else of 16.  8 heads of 128 in 8 bits, write and read: 1,000 tokens
-// 6.0 and 5.9 us with 64, 4.8 and 5.4 with 16; 4,000 7.9 and 7.5 against 7.7 and 7.4; 8,000 11.8 and 9.6 against 12.4 and 11.8.
+// Tiles of 64 tokens where they fill the GPU twice, else of 16.  8 heads of 128 in 8 bits, write and read of tokens from a
+// group's start: 1,000 tokens 6.1 and 5.7 us with 64, 4.9 and 5.1 with 16; 4,000 9.4 and 8.1 against 9.5 and 7.8; 8,000 14.0 and
+// 10.2 against 14.2 and 12.5.  Written from inside a group, where smaller tiles cut more runs: 6.8 against 7.0, 11.6 against
+// 17.5, 17.9 against 27.8.
 template <class Row, class Store, int LANES>
 static hipError_t launch_cache(bool write, const CacheArgs &a, hipStream_t stream)
 {

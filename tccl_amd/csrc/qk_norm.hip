@@ -12,7 +12,8 @@
 // source; the mean is a reduction over head_dim / 8 lanes in registers.  Angles are formed in fp64 turns
 // (fp32 would lose the fraction of a far position's angle) once per token by the workgroup, into LDS.
 // Measured: forward, 4,099 tokens of 48 heads of 128, 8 bf16 sources 78 us, 5.8 TB/s; 8,191 tokens of 20 heads of 256, one
-// fp32 source 63 us, 5.3 TB/s read and written; backward, 8,192 tokens of 48 heads of 128, one bf16 source 52 us, 5.6 TB/s.
+// fp32 source 63 us, 5.3 TB/s read and written; backward, 8,192 tokens of 48 heads of 128, one bf16 source 52 to 53 us, 5.4 TB/s;
+// 777 tokens of 36 heads of 64, four fp32 sources 11.8 us, 2.9 TB/s: five items for four waves, one of which works twice.
 #include <type_traits>
 
 #include "host.h"
