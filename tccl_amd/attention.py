@@ -325,8 +325,8 @@ def decode_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tenso
     Returns ``[batch, q_heads, head_dim]`` bfloat16 and, with ``return_lse`` or ``lse``, the logarithm of the softmax's
     sum, float32 ``[batch, q_heads]``: what ``attention_all_reduce`` joins parts with.  A sequence without tokens gives
     0 and -inf.  Scores, softmax and sums are fp32; an infinite cached value gives NaN, and so may finite ones whose sum,
-    weighted by up to 1 each, passes fp32's range before it is divided.  ``out`` may be q itself where q is contiguous;
-    otherwise outputs must not overlap inputs."""
+    weighted by up to 1 each, passes fp32's range before it is divided.  ``out`` may be q itself where q is contiguous and
+    no other rank's call reads it; otherwise outputs must not overlap inputs."""
     batch, dim, device = lengths.numel(), cache.head_dim, cache.device
     if q.dtype != torch.bfloat16 or q.dim() != 3 or q.shape[0] != batch or q.shape[2] != dim or q.device != device:
         raise ValueError(f"q must be a bfloat16 tensor of shape [{batch}, q_heads, {dim}] on {device}")
