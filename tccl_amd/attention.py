@@ -133,8 +133,9 @@ def qk_norm_rope(tensor: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.T
     turns the first ``2 * len(inv_freq)`` elements (a multiple of 16) in pairs (i, i + half), or (2i, 2i + 1) if
     ``interleaved``, by ``positions[t] * inv_freq[i]``: positions are int64, inv_freq float64, and the angle is reduced
     in fp64, so that far positions keep their precision.  Value heads are only summed.  Everything is fp32 and rounded
-    once.  ``eps`` may be 0, where a head of zeros has no norm and gives NaN.  Returns q, k, v as
-    ``[tokens, heads, head_dim]``.
+    once.  ``eps`` may be 0, where a head of zeros has no norm and gives NaN.  A head whose sum of squares passes fp32's
+    range (elements of about 2^61 and more) becomes 0, with gradients of 0; for eps = 0 one below it loses its norm.
+    Returns q, k, v as ``[tokens, heads, head_dim]``.
 
     With a group of one rank it is the plain norm and rotation."""
     dim = q_weight.numel()

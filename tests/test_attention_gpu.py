@@ -289,6 +289,31 @@ def test_qk_norm_rope_special_values():
     assert torch.isfinite(q[3, 2]).all() and v[3, 0, 0] == math.inf and torch.isfinite(v[3, 0, 1:]).all()
 
 
+@pytest.mark.parametrize("power", [-60, 0, 58])
+def test_qk_norm_rope_of_small_and_large_rows(power):
+    """Every size of row whose sum of squares fp32 holds is normed as well as any other, forward and backward, for eps = 0."""
+    heads, dim = (3, 1, 1), 64
+    parts, w, positions, inv_freq, grads = norm_inputs(1, 5, heads, dim, dim, F32, seed=19)
+    parts = [p * 2.0 ** power for p in parts]
+    group = world_of(parts)
+    dev = [t.to(DEV) for t in (*w, positions, inv_freq)]
+    check_forward(tccl_amd.qk_norm_rope(group.tensor(0), *dev, 3, 1, eps=0.0), parts, w, positions, inv_freq, heads, 0.0, False)
+    got = tccl_amd.qk_norm_rope_backward(*(g.to(DEV) for g in grads), group.tensor(0), *dev, eps=0.0)
+    check_backward(got, parts, w, positions, inv_freq, grads, heads, 0.0, False, sum(heads))
+
+
+def test_qk_norm_rope_of_rows_beyond_fp32():
+    parts, w, positions, inv_freq, grads = norm_inputs(1, 3, (2, 1, 0), 64, 64, F32, seed=20)
+    x = parts[0].view(3, 3, 64)
+    x[1, 1] *= 2.0 ** 70
+    group = world_of(parts)
+    dev = [t.to(DEV) for t in (*w, positions, inv_freq)]
+    q, _, _ = tccl_amd.qk_norm_rope(group.tensor(0), *dev, 2, 1)
+    assert not q[1, 1].any() and q[1, 0].any() and torch.isfinite(q).all()
+    got = tccl_amd.qk_norm_rope_backward(*(g.to(DEV) for g in grads), group.tensor(0), *dev)
+    assert not got[0].view(3, 3, 64)[1, 1].any() and all(torch.isfinite(t).all() for t in got)
+
+
 def test_norm_without_tokens_and_with_a_prefix_view():
     parts, w, positions, inv_freq, _ = norm_inputs(2, 8, (2, 1, 1), 64, 64, BF16)
     group = world_of(parts)
